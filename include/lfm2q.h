@@ -223,6 +223,75 @@ int lfm2q_decode_attention_split_noalloc(const uint16_t *q, const uint16_t *kc, 
                                          const int64_t *pos, uint16_t *out, int B, int NQ, int NKV, int max_len, int S,
                                          float scale, void *stream);
 
+/* ------------------------------------------------------------------ batches of requests over a paged cache
+ * No counterparts in the reference, whose decode step (src/lfm2opt/runtime.py:247-294) runs one sequence over a dense
+ * cache and takes the argmax. One decode iteration of a batch: kv_slots, then per attention layer
+ * qk_norm_rope_kv_paged and tree_attention, then sample_next on the logits (lfm2opt.batch_step.BatchDecodeStep).
+ *
+ * Cache: kc / vc [num_pages, NKV, page, D]. Position t of request b lies on page table[b][t / page], row t % page; its
+ * slot is table[b][t / page] * page + t % page. page = max_len and table[b] = {b} is the dense cache of
+ * lfm2q_decode_attention_split. Every integer array is on the device; dtype is that of every uint16_t tensor. */
+typedef enum { LFM2Q_BF16 = 0, LFM2Q_FP16 = 1, LFM2Q_FP32 = 2 } lfm2q_dtype;
+
+/* Block tables and slot maps from request lengths. Request b holds lens[b] positions and asks for new_lens[b]: it grows
+ * (admission: lens 0), shrinks (rejected drafts) or ends (new_lens 0). Pages come off the top of a stack, free_pages
+ * [num_pages] with n_free[0] entries, and go back onto it.
+ *   A request is granted if both lengths lie in [0, max_pages * page] and, where it needs pages (or brings tokens), the
+ *   sum of pages (tokens) that the valid requests up to it need does not exceed n_free[0] (capacity). got[b] =
+ *   new_lens[b] if granted, else lens[b] (a refused request changes nothing). The granted requests' i-th new page (in
+ *   order of requests, then of pages) is free_pages[n_free - 1 - i], P in all; their i-th returned page, R in all, goes
+ *   to free_pages[n_free - P + R - 1 - i], and its table entry becomes -1; n_free becomes n_free - P + R. (Pages
+ *   returned in a call serve the next one. Growing and shrinking back restores the stack.)
+ *   cu [B + 1]: exclusive sums of the granted tokens, max(0, new_lens - lens); token i of request b is row cu[b] + i of
+ *   positions (lens[b] + i) and slots. Rows from cu[B] on are left as they were.
+ * The tables must hold what earlier calls put there (pages of the pool, each once): entries are moved, not checked.
+ * Needs max_pages * page <= 2^30, num_pages <= 2^30, capacity <= 2^30; got must be neither lens nor new_lens. */
+int lfm2q_kv_slots(const int32_t *lens, const int32_t *new_lens, int32_t *table, int32_t *free_pages, int32_t *n_free,
+                   int32_t *got, int32_t *cu, int64_t *positions, int64_t *slots, int B, int max_pages, int num_pages,
+                   int page, int64_t capacity, void *stream);
+
+/* Per-head RMSNorm of q and k (qw, kw [D], or both NULL: none), rotary positions, k and v into the paged cache.
+ * qkv [N, (NQ + 2 NKV) * D] (q | k | v heads), rows row_stride elements apart (a multiple of 8); D 64 or 128.
+ * The first rot_dim dims of a head turn (a multiple of 16), the rest pass: pair i < rot_dim / 2 by the angle
+ * positions[n] * inv_freq[i] (formed in fp64), cos and sin times scaling. Pairs are dims (i, i + rot_dim / 2), or
+ * (2i, 2i + 1) if interleaved. lfm2opt.rope.inv_freq makes the tables (plain, linear, NTK, YaRN, Llama 3). fp32
+ * throughout, one rounding at the end (lfm2q_qk_norm_rope_kv, the reference's form, rounds at every step).
+ * q_out [N, NQ, D]; k (turned) and v (unchanged) go to cache slot slots[n]; a slot outside [0, num_pages * page), -1 for
+ * one, writes neither. Slots of one call must differ; q_out must not overlap qkv. */
+int lfm2q_qk_norm_rope_kv_paged(const uint16_t *qkv, int64_t row_stride, const uint16_t *qw, const uint16_t *kw,
+                                const float *inv_freq, int rot_dim, float scaling, const int64_t *positions,
+                                const int64_t *slots, uint16_t *q_out, uint16_t *kc, uint16_t *vc, int dtype, int N,
+                                int NQ, int NKV, int D, int num_pages, int page, float eps, int interleaved,
+                                void *stream);
+
+/* Attention of drafted tokens over the paged cache. Request b brings the queries cu[b] .. cu[b + 1] of q [N, NQ, D] (1 to
+ * max_q <= 64 of them: a tree, a chain, or one token), whose keys and values lie at its positions ctx[b] + j. Query i
+ * sees every position < ctx[b], and ctx[b] + j where bit j of mask[cu[b] + i] is set (mask NULL: j <= i). out [N, NQ, D]
+ * = softmax(scale q.k) v; a query that sees nothing gives zeros. Rows outside the requests, and those past max_q of a
+ * request, are left as they were. NQ = G NKV, G <= 64; D 64 or 128; scale > 0. A position whose page is outside
+ * [0, num_pages), or past the table, is not seen.
+ * S splits over the positions (lfm2q_tree_attention_splits suggests a number): with S > 1 ws fp32 [N, NQ, S, D + 2]
+ * holds (m, l, acc[D]) of each (no value needs to be set before; concurrent calls need their own); S = 1 needs none. */
+int lfm2q_tree_attention(const uint16_t *q, const uint16_t *kc, const uint16_t *vc, const int32_t *table,
+                         const int32_t *ctx, const int32_t *cu, const int64_t *mask, uint16_t *out, float *ws,
+                         int dtype, int N, int B, int NQ, int NKV, int D, int num_pages, int page, int max_pages, int S,
+                         int max_q, float scale, void *stream);
+/* The split count (>= 1) that fills the current device for B requests of up to max_q queries and max_len positions.
+ * Not a status. */
+int lfm2q_tree_attention_splits(int B, int NQ, int NKV, int D, int max_q, int max_len);
+
+/* Sampling from given uniforms, the counterpart of lfm2q_argmax_next. Per row of logits [B, V] (dtype, rows row_stride
+ * elements apart, any alignment of rows): temperature T > 0: w_i = e^((x_i - max) / T); in the order (x descending,
+ * index ascending) the first top_k are kept (0 or less: all), of those the shortest prefix whose mass reaches top_p of
+ * theirs (>= 1 or NaN: all; always at least one), of those w_i >= min_p (of the largest, 1). tok[b] = the first index
+ * whose running kept mass, in index order, exceeds u[b] (in [0, 1)) times the kept mass. T <= 0 or NaN, a NaN among the
+ * logits, or no finite one: the argmax, as lfm2q_argmax_next. A NULL temperature, top_k, top_p or min_p [B] is off
+ * (temperature 1). Weights are summed as integers in steps of 2^-44 of the largest: the same token in any launch
+ * shape. pos[0] += 1 if pos is not NULL. V <= 262144. */
+int lfm2q_sample_next(const void *logits, int dtype, int64_t row_stride, const float *temperature, const int32_t *top_k,
+                      const float *top_p, const float *min_p, const float *u, int64_t *tok, int64_t *pos, int B, int V,
+                      void *stream);
+
 /* Replace set_pdl / set_gemv_impl (kernels/lfm2_decode.cpp:165-166). set_pdl toggles Programmatic Dependent
  * Launch for the GEMV kernels (default on). set_gemv_impl is accepted for compatibility; this build has one
  * GEMV implementation. */

@@ -412,4 +412,101 @@ int lfm2q_decode_attention_split_noalloc(const uint16_t *q, const uint16_t *kc, 
                   "decode_attention_split_noalloc");
 }
 
+// ------------------------------------------------------------------ batches of requests over a paged cache
+int lfm2q_kv_slots(const int32_t *lens, const int32_t *new_lens, int32_t *table, int32_t *free_pages, int32_t *n_free,
+                   int32_t *got, int32_t *cu, int64_t *positions, int64_t *slots, int B, int max_pages, int num_pages,
+                   int page, int64_t capacity, void *stream) {
+  REQUIRE(B >= 0 && max_pages > 0 && num_pages > 0 && page > 0,
+          "table [B, max_pages], free_pages [num_pages]: need B >= 0, max_pages, num_pages, page > 0");
+  REQUIRE((long long)max_pages * page <= (1ll << 30) && (long long)num_pages <= (1ll << 30),
+          "max_pages * page and num_pages must be <= 2^30");
+  REQUIRE(B <= (1 << 24), "B must be <= 2^24");
+  REQUIRE(capacity >= 0 && capacity <= (1ll << 30), "positions / slots [capacity]: need 0 <= capacity <= 2^30");
+  REQUIRE(free_pages && n_free && cu && (B == 0 || (lens && new_lens && table && got)) &&
+              (capacity == 0 || (positions && slots)),
+          "every pointer must be non-null");
+  REQUIRE(B == 0 || (got != new_lens && got != lens), "got must be neither lens nor new_lens");
+  if (int e = device_gate()) return e;
+  return launched(launch_kv_slots(lens, new_lens, table, free_pages, n_free, got, cu, positions, slots, B, max_pages,
+                                  num_pages, page, capacity, g_pdl.load(), (cudaStream_t)stream),
+                  "kv_slots");
+}
+
+static int check_half(int dtype, int D) {
+  REQUIRE(dtype == LFM2Q_BF16 || dtype == LFM2Q_FP16, "dtype must be LFM2Q_BF16 or LFM2Q_FP16");
+  REQUIRE(D == 64 || D == 128, "head_dim 64 or 128 only");
+  return LFM2Q_OK;
+}
+
+int lfm2q_qk_norm_rope_kv_paged(const uint16_t *qkv, int64_t row_stride, const uint16_t *qw, const uint16_t *kw,
+                                const float *inv_freq, int rot_dim, float scaling, const int64_t *positions,
+                                const int64_t *slots, uint16_t *q_out, uint16_t *kc, uint16_t *vc, int dtype, int N,
+                                int NQ, int NKV, int D, int num_pages, int page, float eps, int interleaved,
+                                void *stream) {
+  if (int e = check_half(dtype, D)) return e;
+  REQUIRE(N >= 0 && NQ > 0 && NKV > 0 && num_pages > 0 && page > 0,
+          "qkv [N, (NQ + 2 NKV) * D], kc / vc [num_pages, NKV, page, D]: need N >= 0 and the others > 0");
+  REQUIRE((long long)NQ + 2ll * NKV <= 65536, "NQ + 2 NKV must be <= 65536");
+  REQUIRE(rot_dim > 0 && rot_dim <= D && rot_dim % 16 == 0, "rot_dim must be a multiple of 16 in [16, D]");
+  REQUIRE(row_stride >= ((long long)NQ + 2ll * NKV) * D && row_stride % 8 == 0,
+          "qkv rows: the stride must be a multiple of 8 and hold (NQ + 2 NKV) * D");
+  if (N == 0) return LFM2Q_OK;
+  REQUIRE(qkv && inv_freq && positions && slots && q_out && kc && vc, "every pointer but qw and kw must be non-null");
+  REQUIRE((qw == nullptr) == (kw == nullptr), "qw and kw: both or neither");
+  REQUIRE(aligned16(qkv) && aligned16(qw) && aligned16(kw) && aligned16(q_out) && aligned16(kc) && aligned16(vc),
+          "qkv, qw, kw, q_out, kc and vc must be 16-byte aligned");
+  if (int e = device_gate()) return e;
+  return launched(launch_qk_norm_rope_kv_paged(qkv, row_stride, qw, kw, inv_freq, rot_dim, scaling, positions, slots,
+                                               q_out, kc, vc, N, NQ, NKV, D, num_pages, page, eps, interleaved != 0,
+                                               dtype == LFM2Q_FP16, g_pdl.load(), (cudaStream_t)stream),
+                  "qk_norm_rope_kv_paged");
+}
+
+int lfm2q_tree_attention_splits(int B, int NQ, int NKV, int D, int max_q, int max_len) {
+  if (B <= 0 || NKV <= 0 || NQ < NKV || max_q <= 0 || max_len <= 0) return 1;
+  return tree_attention_splits(B, NQ, NKV, D, max_q, max_len);
+}
+
+int lfm2q_tree_attention(const uint16_t *q, const uint16_t *kc, const uint16_t *vc, const int32_t *table,
+                         const int32_t *ctx, const int32_t *cu, const int64_t *mask, uint16_t *out, float *ws,
+                         int dtype, int N, int B, int NQ, int NKV, int D, int num_pages, int page, int max_pages, int S,
+                         int max_q, float scale, void *stream) {
+  if (int e = check_half(dtype, D)) return e;
+  REQUIRE(N >= 0 && B >= 0 && NKV > 0 && num_pages > 0 && page > 0 && max_pages > 0,
+          "q [N, NQ, D], kc / vc [num_pages, NKV, page, D], table [B, max_pages]: need N, B >= 0 and the others > 0");
+  REQUIRE(NQ > 0 && NQ % NKV == 0 && NQ / NKV <= 64, "NQ must be a multiple of NKV, at most 64 times it");
+  REQUIRE(max_q >= 1 && max_q <= 64, "max_q (drafted tokens of a request) must be in [1, 64]");
+  REQUIRE((long long)max_pages * page <= (1ll << 30), "max_pages * page must be <= 2^30");
+  REQUIRE(B <= 65535 && (long long)B * NKV <= 0x7fffffffLL, "B must be <= 65535");
+  REQUIRE(S >= 1 && S <= 65535, "ws [N, NQ, S, D + 2]: need 1 <= S <= 65535");
+  REQUIRE(scale > 0.f && scale < 1e30f, "scale must be positive and finite");
+  if (N == 0 || B == 0) return LFM2Q_OK;
+  REQUIRE(q && kc && vc && table && ctx && cu && out, "q, kc, vc, table, ctx, cu and out must be non-null");
+  REQUIRE(S == 1 || ws, "ws must be non-null when S > 1");
+  REQUIRE(aligned16(q) && aligned16(kc) && aligned16(vc) && aligned16(out) && aligned16(ws),
+          "q, kc, vc, out and ws must be 16-byte aligned");
+  if (int e = device_gate()) return e;
+  return launched(launch_tree_attention(q, kc, vc, table, ctx, cu, mask, out, ws, N, B, NQ, NKV, D, num_pages, page,
+                                        max_pages, S, max_q, scale, dtype == LFM2Q_FP16, g_pdl.load(),
+                                        (cudaStream_t)stream),
+                  "tree_attention");
+}
+
+int lfm2q_sample_next(const void *logits, int dtype, int64_t row_stride, const float *temperature, const int32_t *top_k,
+                      const float *top_p, const float *min_p, const float *u, int64_t *tok, int64_t *pos, int B, int V,
+                      void *stream) {
+  REQUIRE(dtype == LFM2Q_BF16 || dtype == LFM2Q_FP16 || dtype == LFM2Q_FP32,
+          "dtype must be LFM2Q_BF16, LFM2Q_FP16 or LFM2Q_FP32");
+  REQUIRE(B >= 0 && B <= 65535 && V > 0 && V <= (1 << 18), "logits [B, V]: need 0 <= B <= 65535 and 0 < V <= 262144");
+  REQUIRE(row_stride >= V, "logits rows: the stride must be >= V");
+  if (B == 0) return LFM2Q_OK;
+  REQUIRE(logits && u && tok, "logits, u and tok must be non-null");
+  REQUIRE(reinterpret_cast<uintptr_t>(logits) % (dtype == LFM2Q_FP32 ? 4 : 2) == 0,
+          "logits must be aligned to their elements");
+  if (int e = device_gate()) return e;
+  return launched(launch_sample_next(logits, dtype, row_stride, temperature, top_k, top_p, min_p, u, tok, pos, B, V,
+                                     g_pdl.load(), (cudaStream_t)stream),
+                  "sample_next");
+}
+
 }  // extern "C"

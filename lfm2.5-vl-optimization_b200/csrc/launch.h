@@ -99,6 +99,41 @@ cudaError_t launch_qk_norm_rope_kv(const void *qkv, const void *qw, const void *
                                    float scaling, const int64_t *pos, void *q_out, void *kc, void *vc, int B, int NQ,
                                    int NKV, int max_len, float eps, bool pdl, cudaStream_t st);
 
+// paged.cu: block tables and slot maps; q/k norm + rotary positions + paged cache write (half: fp16, else bf16)
+cudaError_t launch_kv_slots(const int *lens, const int *want, int *table, int *freelist, int *n_free, int *got, int *cu,
+                            int64_t *positions, int64_t *slots, int B, int width, int pool, int page,
+                            long long capacity, bool pdl, cudaStream_t st);
+cudaError_t launch_qk_norm_rope_kv_paged(const void *qkv, long long row_stride, const void *qw, const void *kw,
+                                         const float *inv_freq, int rot, float scaling, const int64_t *positions,
+                                         const int64_t *slots, void *q_out, void *kc, void *vc, int N, int NQ, int NKV,
+                                         int D, long long num_pages, int page, float eps, bool interleaved, bool half,
+                                         bool pdl, cudaStream_t st);
+
+// tree_attention.cu: drafted tokens over the paged cache (half: fp16, else bf16); ws is read and written where S > 1
+int tree_attention_splits(int B, int NQ, int NKV, int D, int max_q, long long max_len);
+cudaError_t launch_tree_attention(const void *q, const void *kc, const void *vc, const int *table, const int *ctx,
+                                  const int *cu, const int64_t *mask, void *out, float *ws, int N, int B, int NQ,
+                                  int NKV, int D, int num_pages, int page, int width, int S, int max_q, float scale,
+                                  bool half, bool pdl, cudaStream_t st);
+
+// sample.cu: sampling with temperature, top-k, top-p and min-p (dtype as lfm2q_dtype)
+cudaError_t launch_sample_next(const void *logits, int dtype, long long stride, const float *temperature,
+                               const int *top_k, const float *top_p, const float *min_p, const float *u, int64_t *tok,
+                               int64_t *pos, int B, int V, bool pdl, cudaStream_t st);
+
+// launch configuration of a programmatic dependent (attr: storage for its one attribute)
+inline cudaLaunchConfig_t pdl_config(dim3 grid, dim3 block, bool pdl, cudaStream_t st, cudaLaunchAttribute *attr) {
+  cudaLaunchConfig_t cfg = {};
+  attr->id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr->val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = pdl ? 1 : 0;
+  return cfg;
+}
+
 // device facts cached per device
 int device_sm_count();
 bool device_is_sm100();

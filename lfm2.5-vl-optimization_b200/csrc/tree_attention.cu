@@ -1,0 +1,527 @@
+// Attention of drafted tokens over a paged KV cache: every request b brings T_b = cu[b + 1] - cu[b] query tokens
+// (a tree of drafts, a chain, or the one token of an ordinary decode step), whose keys and values already lie in the
+// cache behind its ctx[b] cached positions. Query i sees every position t < ctx[b], and position ctx[b] + j (draft j)
+// where bit j of its mask is set (mask NULL: j <= i). out = softmax(scale q.k) v per head; a query that sees nothing
+// gives zeros. Heads are grouped: G = NQ / NKV query heads share a KV head.
+//
+// Mathematics: the rows of one (request, KV head) are its T_b G queries, so K and V are read once for all of them;
+// the online softmax keeps a running maximum m and sum l per row in fp32 (base 2: scores times scale log2 e) and
+// rescales the fp32 accumulator when m grows. The probabilities are rounded to the cache's type for the second
+// product, and l sums the unrounded ones: each p is off by at most half a step, which leaves out within one rounding
+// of that type.
+//
+// A block takes a tile of 64 keys at a time through a ring of cp.async stages (rows swizzled in 16-byte units, so
+// ldmatrix reads are conflict-free), mma.sync m16n8k16 for both products. Long caches are cut into S splits, each at
+// most ceil(len / S) keys rounded up to the tile; the partial (m, l, acc) of a split goes to ws and a second kernel
+// joins them in split order. Rows behind the request's length, and positions whose table entry is not a page of the
+// pool, are filled with zeros in shared memory and masked: nothing outside the pool is read.
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <atomic>
+#include <cstdint>
+
+#include "common.cuh"
+#include "launch.h"
+
+namespace lfm2q {
+namespace {
+
+constexpr int TA_KEYS = 64;  // keys per tile
+
+template <class T>
+struct Mma;
+template <>
+struct Mma<bf16> {
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
+  static __device__ __forceinline__ float2 up2(uint32_t u) { return make_float2(bf_lo(u), bf_hi(u)); }
+  static __device__ __forceinline__ bool finite2(uint32_t u) {
+    return (u & 0x7f80u) != 0x7f80u && (u & 0x7f800000u) != 0x7f800000u;
+  }
+};
+template <>
+struct Mma<__half> {
+  static __device__ __forceinline__ void run(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&h);
+  }
+  static __device__ __forceinline__ float2 up2(uint32_t u) { return __half22float2(*reinterpret_cast<__half2 *>(&u)); }
+  static __device__ __forceinline__ bool finite2(uint32_t u) {
+    return (u & 0x7c00u) != 0x7c00u && (u & 0x7c000000u) != 0x7c000000u;
+  }
+};
+
+__device__ __forceinline__ uint32_t saddr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+__device__ __forceinline__ void ldsm4t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a));
+}
+// 16 bytes global -> shared; bytes = 0 writes zeros and reads nothing
+__device__ __forceinline__ void cp16(uint32_t dst, const void *src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+// 2^x, to about 2 ulp (x <= 0 here; results below 2^-126 are 0)
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+struct TreeArgs {
+  const void *q, *kc, *vc;
+  const int *table, *ctx, *cu;
+  const unsigned long long *mask;
+  void *out;
+  float *ws;
+  float scale_log2;  // scale * log2 e
+  int N, NQ, NKV, G, page, width, num_pages, S, max_q;
+};
+
+// Lengths of request b, held inside what the tensors have: queries within [0, N) and at most max_q, positions within
+// the table.
+struct Request {
+  int n0, T, ctx, len;
+  __device__ __forceinline__ Request(const TreeArgs &a, int b) {
+    const int c0 = __ldcg(a.cu + b), c1 = __ldcg(a.cu + b + 1);
+    n0 = min(max(c0, 0), a.N);
+    T = max(0, min(min(c1, a.N) - n0, a.max_q));
+    const long long room = (long long)a.width * a.page;
+    ctx = (int)min((long long)max(0, __ldcg(a.ctx + b)), room);
+    len = (int)min((long long)ctx + T, room);
+  }
+};
+
+// WM x WK warps: WM row groups of 16 MT rows, WK groups of 64 / WK keys of every tile (joined at the end).
+template <class T, int D, int WM, int WK, int MT, int STAGES>
+__global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
+  constexpr int THREADS = 32 * WM * WK, ROWS = 16 * WM * MT;
+  constexpr int CH = D / 8;              // 16-byte units per row
+  constexpr int KW = TA_KEYS / WK;       // keys of a tile per warp
+  constexpr int NB = KW / 8;             // 8-key column blocks per warp
+  constexpr int TILE = TA_KEYS * D * 2;  // bytes of a K (or V) tile
+  extern __shared__ __align__(128) uint8_t ta_smem[];
+  __shared__ int bad_pages;  // a page outside the pool was met
+  uint8_t *sk = ta_smem, *sv = ta_smem + STAGES * TILE, *sq = ta_smem + 2 * STAGES * TILE;
+  pdl_trigger();
+  pdl_wait();
+  const int kvh = blockIdx.x % a.NKV, b = blockIdx.x / a.NKV, split = blockIdx.y, r_base = blockIdx.z * ROWS;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, wm = warp / WK, wk = warp % WK;
+  const Request rq(a, b);
+  const int rows = rq.T * a.G;
+  if (r_base >= rows) return;
+  const int chunk = ((rq.len + a.S - 1) / a.S + TA_KEYS - 1) / TA_KEYS * TA_KEYS;
+  const int t0 = min((long long)split * chunk, (long long)rq.len), t1 = min(rq.len, t0 + chunk);
+  const int tiles = (t1 - t0 + TA_KEYS - 1) / TA_KEYS;
+  if (tid == 0) bad_pages = 0;
+  __syncthreads();
+
+  // queries: row r = token r / G, head kvh G + r % G, swizzled like the keys; rows past the end are zeros
+  for (int i = tid; i < ROWS * CH; i += THREADS) {
+    const int r = i / CH, c = i % CH, gr = r_base + r;
+    const bool in = gr < rows;
+    const T *src = reinterpret_cast<const T *>(a.q) +
+                   ((size_t)(rq.n0 + (in ? gr / a.G : 0)) * a.NQ + kvh * a.G + (in ? gr % a.G : 0)) * D + 8 * c;
+    cp16(saddr(sq + (r * CH + (c ^ (r & 7))) * 16), src, in ? 16 : 0);
+  }
+  cp_commit();
+
+  const int *table = a.table + (size_t)b * a.width;
+  auto page_of = [&](int t) { return __ldcg(table + t / a.page); };
+  auto load_tile = [&](int i) {
+    const int base = t0 + i * TA_KEYS, slot = i % STAGES;
+    constexpr int RPP = THREADS / CH;  // rows per pass
+    static_assert(THREADS % CH == 0 && TA_KEYS % RPP == 0, "whole passes");
+    const int c = tid % CH;
+#pragma unroll
+    for (int p = 0; p < TA_KEYS / RPP; ++p) {
+      const int r = p * RPP + tid / CH, t = base + r;
+      bool in = t < t1;
+      size_t off = 0;
+      if (in) {
+        const int pg = page_of(t);
+        in = pg >= 0 && pg < a.num_pages;
+        if (!in) bad_pages = 1;
+        else off = (((size_t)pg * a.NKV + kvh) * a.page + t % a.page) * D + 8 * c;
+      }
+      const uint32_t d = (r * CH + (c ^ (r & 7))) * 16;
+      cp16(saddr(sk + slot * TILE + d), reinterpret_cast<const T *>(a.kc) + off, in ? 16 : 0);
+      cp16(saddr(sv + slot * TILE + d), reinterpret_cast<const T *>(a.vc) + off, in ? 16 : 0);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+    if (i < tiles) load_tile(i);
+    cp_commit();
+  }
+
+  float o[MT][D / 8][4], m[MT][2], l[MT][2];
+  unsigned long long see[MT][2];  // the drafts that the lane's rows see
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+    for (int j = 0; j < D / 8; ++j) o[mt][j][0] = o[mt][j][1] = o[mt][j][2] = o[mt][j][3] = 0.f;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      m[mt][h] = -INFINITY;
+      l[mt][h] = 0.f;
+      const int gr = r_base + wm * 16 * MT + mt * 16 + (lane >> 2) + 8 * h;
+      see[mt][h] = 0;
+      if (gr < rows) {
+        const int i = gr / a.G;
+        see[mt][h] = a.mask ? __ldcg(a.mask + rq.n0 + i) : (i >= 63 ? ~0ull : (2ull << i) - 1);
+      }
+    }
+  }
+
+  for (int it = 0; it < tiles; ++it) {
+    cp_wait<STAGES - 2>();
+    __syncthreads();  // the tile has landed for every warp, and the slot of tile it - 1 is free
+    if (it + STAGES - 1 < tiles) load_tile(it + STAGES - 1);
+    cp_commit();
+    const int slot = it % STAGES, base = t0 + it * TA_KEYS;
+    const uint32_t kb = saddr(sk + slot * TILE), vb = saddr(sv + slot * TILE), qb = saddr(sq);
+    const int k0 = wk * KW;  // this warp's keys of the tile
+
+    // ---------------------------------------------------------------- scores
+    float s[MT][NB][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int j = 0; j < NB; ++j) s[mt][j][0] = s[mt][j][1] = s[mt][j][2] = s[mt][j][3] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      uint32_t qa[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        const int r = wm * 16 * MT + mt * 16 + (lane & 15), c = 2 * kk + (lane >> 4);
+        ldsm4(qa[mt], qb + (r * CH + (c ^ (r & 7))) * 16);
+      }
+#pragma unroll
+      for (int jp = 0; jp < NB / 2; ++jp) {  // two 8-key blocks per ldmatrix.x4
+        uint32_t kf[4];
+        const int r = k0 + jp * 16 + (lane & 7) + ((lane >> 4) << 3), c = 2 * kk + ((lane >> 3) & 1);
+        ldsm4(kf, kb + (r * CH + (c ^ (r & 7))) * 16);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          Mma<T>::run(s[mt][2 * jp], qa[mt], kf[0], kf[1]);
+          Mma<T>::run(s[mt][2 * jp + 1], qa[mt], kf[2], kf[3]);
+        }
+      }
+    }
+    // ---------------------------------------------------------------- masks
+    const bool edge = base + TA_KEYS > rq.ctx || base + TA_KEYS > t1;
+    const bool bad = *(volatile int *)&bad_pages != 0;
+    if (edge || bad) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int t = base + k0 + 8 * j + 2 * (lane & 3) + e;
+          bool in = t < t1;
+          if (in && bad) {
+            const int pg = page_of(t);
+            in = pg >= 0 && pg < a.num_pages;
+          }
+          const int d = t - rq.ctx;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              if (!in || (d >= 0 && !((see[mt][h] >> d) & 1))) s[mt][j][2 * h + e] = -INFINITY;
+        }
+    }
+    // ---------------------------------------------------------------- online softmax
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float mx = -INFINITY;
+#pragma unroll
+        for (int j = 0; j < NB; ++j) mx = fmaxf(mx, fmaxf(s[mt][j][2 * h], s[mt][j][2 * h + 1]));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m[mt][h], mx * a.scale_log2);
+        const float ms = mn == -INFINITY ? 0.f : mn;
+        const float corr = ex2(m[mt][h] - ms);  // 2^-inf = 0 while nothing was seen
+        m[mt][h] = mn;
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < NB; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float p = ex2(fmaf(s[mt][j][2 * h + e], a.scale_log2, -ms));
+            s[mt][j][2 * h + e] = p;
+            sum += p;
+          }
+        l[mt][h] = l[mt][h] * corr + sum;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          o[mt][j][2 * h] *= corr;
+          o[mt][j][2 * h + 1] *= corr;
+        }
+      }
+    // ---------------------------------------------------------------- values
+    // A draft that a row does not see has p = 0 there, but 0 times an infinity or a NaN is a NaN: drafts whose value
+    // row holds one are taken out of the product and added row by row where they are seen.
+    unsigned long long weird = 0;
+    if (base + TA_KEYS > rq.ctx) {
+#pragma unroll
+      for (int g = 0; g < (KW + 31) / 32; ++g) {
+        bool w = false;
+        const int r = k0 + g * 32 + lane;
+        if (g * 32 + lane < KW) {
+#pragma unroll 4
+          for (int c = 0; c < CH; ++c) {
+            const uint4 u = *reinterpret_cast<const uint4 *>(sv + slot * TILE + (r * CH + c) * 16);
+            w = w || !(Mma<T>::finite2(u.x) && Mma<T>::finite2(u.y) && Mma<T>::finite2(u.z) && Mma<T>::finite2(u.w));
+          }
+        }
+        weird |= (unsigned long long)__ballot_sync(0xffffffffu, w) << (32 * g);
+      }
+      for (unsigned long long left = weird; left; left &= left - 1) {
+        const int c = __ffsll(left) - 1, t = base + k0 + c, d = t - rq.ctx;
+        const int from = (lane & ~3) | ((c & 7) >> 1);
+        const uint32_t *vr = reinterpret_cast<const uint32_t *>(sv + slot * TILE) + (k0 + c) * CH * 4 + (lane & 3);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            float p = 0.f;
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+              if (j == (c >> 3)) p = (c & 1) ? s[mt][j][2 * h + 1] : s[mt][j][2 * h];
+            p = __shfl_sync(0xffffffffu, p, from);
+            if (t < t1 && (d < 0 || ((see[mt][h] >> d) & 1))) {
+#pragma unroll
+              for (int j = 0; j < D / 8; ++j) {
+                const uint32_t u = vr[(j ^ ((k0 + c) & 7)) * 4];
+                const float2 v = Mma<T>::up2(u);
+                o[mt][j][2 * h] += p * v.x;
+                o[mt][j][2 * h + 1] += p * v.y;
+              }
+            }
+          }
+      }
+    }
+#pragma unroll
+    for (int kk = 0; kk < KW / 16; ++kk) {
+      uint32_t pa[MT][4];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        pa[mt][0] = Mma<T>::pack(s[mt][2 * kk][0], s[mt][2 * kk][1]);
+        pa[mt][1] = Mma<T>::pack(s[mt][2 * kk][2], s[mt][2 * kk][3]);
+        pa[mt][2] = Mma<T>::pack(s[mt][2 * kk + 1][0], s[mt][2 * kk + 1][1]);
+        pa[mt][3] = Mma<T>::pack(s[mt][2 * kk + 1][2], s[mt][2 * kk + 1][3]);
+      }
+#pragma unroll
+      for (int jp = 0; jp < D / 16; ++jp) {
+        uint32_t vf[4];
+        const int r = k0 + kk * 16 + (lane & 15), c = 2 * jp + (lane >> 4);
+        ldsm4t(vf, vb + (r * CH + (c ^ (r & 7))) * 16);
+        if (weird) {  // a lane's registers hold keys 2 (lane % 4), + 1 of each eight
+          const uint32_t w = (uint32_t)(weird >> (16 * kk + 2 * (lane & 3)));
+          const uint32_t k0m = ((w & 1) ? 0u : 0xffffu) | ((w & 2) ? 0u : 0xffff0000u);
+          const uint32_t k8m = ((w & 0x100) ? 0u : 0xffffu) | ((w & 0x200) ? 0u : 0xffff0000u);
+          vf[0] &= k0m;
+          vf[1] &= k8m;
+          vf[2] &= k0m;
+          vf[3] &= k8m;
+        }
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          Mma<T>::run(o[mt][2 * jp], pa[mt], vf[0], vf[1]);
+          Mma<T>::run(o[mt][2 * jp + 1], pa[mt], vf[2], vf[3]);
+        }
+      }
+    }
+  }
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 1);
+      l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 2);
+    }
+
+  // ---------------------------------------------------------------- join the WK key groups of a row group
+  if (WK > 1) {
+    constexpr int PITCH = D + 4;  // floats per row: m, l, acc (4 floats apart from a bank multiple)
+    static_assert(WM * WK * 16 * MT * PITCH * 4 <= 2 * STAGES * TILE, "the partials fit in the ring");
+    float *part = reinterpret_cast<float *>(ta_smem);
+    cp_wait<0>();
+    __syncthreads();
+    if (wk > 0) {
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float *p = part + ((wm * WK + wk) * 16 * MT + mt * 16 + (lane >> 2) + 8 * h) * PITCH;
+          if ((lane & 3) == 0) {
+            p[D] = m[mt][h];
+            p[D + 1] = l[mt][h];
+          }
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j)
+            *reinterpret_cast<float2 *>(p + 8 * j + 2 * (lane & 3)) = make_float2(o[mt][j][2 * h], o[mt][j][2 * h + 1]);
+        }
+    }
+    __syncthreads();
+    if (wk > 0) return;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        for (int w = 1; w < WK; ++w) {
+          const float *p = part + ((wm * WK + w) * 16 * MT + mt * 16 + (lane >> 2) + 8 * h) * PITCH;
+          const float m2 = p[D], l2 = p[D + 1], mn = fmaxf(m[mt][h], m2), ms = mn == -INFINITY ? 0.f : mn;
+          const float c1 = ex2(m[mt][h] - ms), c2 = ex2(m2 - ms);
+          m[mt][h] = mn;
+          l[mt][h] = l[mt][h] * c1 + l2 * c2;
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) {
+            const float2 v = *reinterpret_cast<const float2 *>(p + 8 * j + 2 * (lane & 3));
+            o[mt][j][2 * h] = o[mt][j][2 * h] * c1 + v.x * c2;
+            o[mt][j][2 * h + 1] = o[mt][j][2 * h + 1] * c1 + v.y * c2;
+          }
+        }
+  }
+
+  // ---------------------------------------------------------------- out, or this split's partial
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int gr = r_base + wm * 16 * MT + mt * 16 + (lane >> 2) + 8 * h;
+      if (gr >= rows) continue;
+      const size_t row = (size_t)(rq.n0 + gr / a.G) * a.NQ + kvh * a.G + gr % a.G;
+      if (a.S == 1) {
+        const float inv = l[mt][h] == 0.f ? 0.f : 1.f / l[mt][h];
+        uint32_t *dst = reinterpret_cast<uint32_t *>(reinterpret_cast<T *>(a.out) + row * D) + (lane & 3);
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) dst[4 * j] = Mma<T>::pack(o[mt][j][2 * h] * inv, o[mt][j][2 * h + 1] * inv);
+      } else {
+        float *w = a.ws + (row * a.S + split) * (D + 2);
+        if ((lane & 3) == 0) *reinterpret_cast<float2 *>(w) = make_float2(m[mt][h], l[mt][h]);
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j)
+          *reinterpret_cast<float2 *>(w + 2 + 8 * j + 2 * (lane & 3)) = make_float2(o[mt][j][2 * h], o[mt][j][2 * h + 1]);
+      }
+    }
+}
+
+// One warp per (query, head): the S partials joined in split order.
+constexpr int TC_WARPS = 4;
+template <class T, int D>
+__global__ void __launch_bounds__(32 * TC_WARPS) tree_combine_kernel(const TreeArgs a) {
+  constexpr int DPL = D / 32;  // dims per lane
+  pdl_trigger();
+  pdl_wait();
+  const int lane = threadIdx.x & 31, unit = blockIdx.x * TC_WARPS + (threadIdx.x >> 5);
+  const int b = blockIdx.y, i = unit / a.NQ, h = unit % a.NQ;
+  const Request rq(a, b);
+  if (i >= rq.T) return;
+  const size_t row = (size_t)(rq.n0 + i) * a.NQ + h;
+  const float *w = a.ws + row * a.S * (D + 2);
+  float M = -INFINITY;
+  for (int s = lane; s < a.S; s += 32) M = fmaxf(M, __ldcg(w + (size_t)s * (D + 2)));
+  M = warp_max(M);
+  const float ms = M == -INFINITY ? 0.f : M;
+  float L = 0.f, acc[DPL];
+#pragma unroll
+  for (int j = 0; j < DPL; ++j) acc[j] = 0.f;
+#pragma unroll 4
+  for (int s = 0; s < a.S; ++s) {
+    const float *p = w + (size_t)s * (D + 2);
+    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p));
+    const float c = ex2(ml.x - ms);
+    L += ml.y * c;
+#pragma unroll
+    for (int j = 0; j < DPL; j += 2) {
+      const float2 v = __ldcg(reinterpret_cast<const float2 *>(p + 2 + DPL * lane + j));
+      acc[j] += v.x * c;
+      acc[j + 1] += v.y * c;
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  uint32_t *dst = reinterpret_cast<uint32_t *>(reinterpret_cast<T *>(a.out) + row * D + DPL * lane);
+#pragma unroll
+  for (int j = 0; j < DPL; j += 2) dst[j / 2] = Mma<T>::pack(acc[j] * inv, acc[j + 1] * inv);
+}
+
+template <class T, int D, int WM, int WK, int MT, int STAGES>
+cudaError_t launch_tile(const TreeArgs &a, int B, bool pdl, cudaStream_t st) {
+  constexpr int ROWS = 16 * WM * MT, SMEM = 2 * STAGES * TA_KEYS * D * 2 + ROWS * D * 2;
+  auto kernel = tree_kernel<T, D, WM, WK, MT, STAGES>;
+  static std::atomic<int> attr_set[64];  // the shared-memory opt-in, once per device
+  int dev = 0;
+  if (const cudaError_t e = cudaGetDevice(&dev)) return e;
+  if (dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
+    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM)) return e;
+    attr_set[dev].store(1, std::memory_order_release);
+  }
+  cudaLaunchAttribute attr;
+  cudaLaunchConfig_t cfg = pdl_config(dim3(B * a.NKV, a.S, (a.max_q * a.G + ROWS - 1) / ROWS), dim3(32 * WM * WK), pdl,
+                                      st, &attr);
+  cfg.dynamicSmemBytes = SMEM;
+  if (const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a)) return e;
+  if (a.S == 1) return cudaSuccess;
+  cfg = pdl_config(dim3((a.max_q * a.NQ + TC_WARPS - 1) / TC_WARPS, B), dim3(32 * TC_WARPS), pdl, st, &attr);
+  return cudaLaunchKernelEx(&cfg, tree_combine_kernel<T, D>, a);
+}
+
+template <class T, int D>
+cudaError_t launch_rows(const TreeArgs &a, int B, bool pdl, cudaStream_t st) {
+  const int rows = a.max_q * a.G;
+  if (rows <= 16) return launch_tile<T, D, 1, 4, 1, 4>(a, B, pdl, st);
+  if (rows <= 32) return launch_tile<T, D, 2, 2, 1, 4>(a, B, pdl, st);
+  if (rows <= 64) return launch_tile<T, D, 4, 1, 1, 3>(a, B, pdl, st);
+  if constexpr (D == 64) return launch_tile<T, D, 4, 1, 2, 3>(a, B, pdl, st);
+  else return launch_tile<T, D, 8, 1, 1, 3>(a, B, pdl, st);  // 128-wide accumulators of 32 rows would spill
+}
+
+}  // namespace
+
+int tree_attention_splits(int B, int NQ, int NKV, int D, int max_q, long long max_len) {
+  // Enough splits to give every SM two blocks, but none shorter than four tiles.
+  const long long rows = (long long)max_q * (NQ / NKV), blocks = (long long)B * NKV * ((rows + 127) / 128);
+  const long long want = (2LL * device_sm_count() + blocks - 1) / blocks;
+  const long long most = (max_len + 4 * TA_KEYS - 1) / (4 * TA_KEYS);
+  (void)D;
+  return (int)std::max(1LL, std::min(std::min(want, most), 64LL));
+}
+
+cudaError_t launch_tree_attention(const void *q, const void *kc, const void *vc, const int *table, const int *ctx,
+                                  const int *cu, const int64_t *mask, void *out, float *ws, int N, int B, int NQ,
+                                  int NKV, int D, int num_pages, int page, int width, int S, int max_q, float scale,
+                                  bool half, bool pdl, cudaStream_t st) {
+  const TreeArgs a{q, kc, vc, table, ctx, cu, reinterpret_cast<const unsigned long long *>(mask), out, ws,
+                   scale * 1.4426950408889634f, N, NQ, NKV, NQ / NKV, page, width, num_pages, S, max_q};
+  if (half) return D == 64 ? launch_rows<__half, 64>(a, B, pdl, st) : launch_rows<__half, 128>(a, B, pdl, st);
+  return D == 64 ? launch_rows<bf16, 64>(a, B, pdl, st) : launch_rows<bf16, 128>(a, B, pdl, st);
+}
+
+}  // namespace lfm2q

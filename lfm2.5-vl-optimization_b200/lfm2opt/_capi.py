@@ -9,11 +9,13 @@ from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "liblfm2q.so"
 
+BF16, FP16, FP32 = 0, 1, 2  # lfm2q_dtype
 OK, EINVAL, ENOTSUP, ECUDA, ETIMEOUT = 0, -22, -95, -5, -62
 
 _p = ctypes.c_void_p
 _i = ctypes.c_int
 _f = ctypes.c_float
+_l = ctypes.c_int64
 
 # name -> argument types (all entry points return int unless listed in _VOID / _STR)
 SIGNATURES = {
@@ -48,6 +50,12 @@ SIGNATURES = {
     "lfm2q_argmax_next": [_p, _p, _p, _i, _i, _p],
     "lfm2q_qk_norm_rope_kv": [_p, _p, _p, _p, _f, _p, _p, _p, _p, _i, _i, _i, _i, _f, _p],
     "lfm2q_decode_attention_split": [_p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _p],
+    "lfm2q_kv_slots": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _l, _p],
+    "lfm2q_qk_norm_rope_kv_paged": [_p, _l, _p, _p, _p, _i, _f, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _f, _i,
+                                    _p],
+    "lfm2q_tree_attention": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p],
+    "lfm2q_tree_attention_splits": [_i, _i, _i, _i, _i, _i],
+    "lfm2q_sample_next": [_p, _i, _l, _p, _p, _p, _p, _p, _p, _p, _i, _i, _p],
     "lfm2q_decode_attention_split_noalloc": [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _p],
 }
 _VOID = {"lfm2q_set_pdl", "lfm2q_set_gemv_impl", "lfm2q_set_gemm_tile", "lfm2q_set_gemv_trigger",

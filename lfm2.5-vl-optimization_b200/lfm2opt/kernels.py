@@ -411,6 +411,126 @@ class DecodeGemvExt:
             _capi.call("lfm2q_decode_attention_split", q.data_ptr(), kc.data_ptr(), vc.data_ptr(), pos.data_ptr(),
                        out.data_ptr(), ws.data_ptr(), B, NQ, NKV, max_len, ws.size(2), float(scale), _stream(q))
 
+    # -------------------------------------------------- batches of requests over a paged cache (include/lfm2q.h)
+    @staticmethod
+    def _same_device(first, *rest):
+        for t in rest:
+            _req(t is None or t.device == first.device, "every tensor must be on one device")
+
+    def kv_slots(self, lens, new_lens, table, free, n_free, page, got, cu, positions, slots):
+        """Block tables and slot maps from request lengths (no counterpart in the reference; lfm2q_kv_slots has the
+        rules). lens, new_lens, got int32 [B], table int32 [B, max_pages], free int32 [num_pages] with n_free int32 [1]
+        entries (a stack), cu int32 [B + 1], positions / slots int64 [capacity]: table, free and n_free are updated in
+        place; got, cu and the first cu[B] rows of positions and slots are written."""
+        for t, n in ((lens, "lens"), (new_lens, "new_lens"), (table, "table"), (free, "free"), (n_free, "n_free"),
+                     (got, "got"), (cu, "cu")):
+            _req(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous(), f"{n} must be contiguous CUDA int32")
+        for t, n in ((positions, "positions"), (slots, "slots")):
+            _req(t.is_cuda and t.dtype == torch.int64 and t.is_contiguous(), f"{n} must be contiguous CUDA int64")
+        B = lens.numel()
+        _req(table.dim() == 2 and table.size(0) == B and table.size(1) > 0, "table [B, max_pages]")
+        _req(new_lens.numel() == B and got.numel() == B and cu.numel() == B + 1 and n_free.numel() == 1,
+             "lens, new_lens, got [B], cu [B + 1], n_free [1]")
+        _req(positions.numel() == slots.numel(), "positions and slots: one length")
+        self._same_device(lens, new_lens, table, free, n_free, got, cu, positions, slots)
+        with _DeviceOf(lens):
+            _capi.call("lfm2q_kv_slots", lens.data_ptr(), new_lens.data_ptr(), table.data_ptr(), free.data_ptr(),
+                       n_free.data_ptr(), got.data_ptr(), cu.data_ptr(), positions.data_ptr(), slots.data_ptr(), B,
+                       table.size(1), free.numel(), int(page), slots.numel(), _stream(lens))
+
+    @staticmethod
+    def _paged(q, kc, vc, name):
+        _req(q.dtype in (_BF, torch.float16), f"{name} must be bf16 or fp16")
+        for t, n in ((kc, "kc"), (vc, "vc")):
+            _req(t.is_cuda and t.dtype == q.dtype and t.is_contiguous() and t.dim() == 4,
+                 f"{n} must be contiguous CUDA [num_pages, NKV, page, D] of {name}'s dtype")
+        _req(vc.shape == kc.shape, "kc and vc: one shape")
+        _req(kc.size(3) in (64, 128), "head_dim 64 or 128 only")
+
+    def qk_norm_rope_kv_paged(self, qkv, qw, kw, inv_freq, scaling, positions, slots, q_out, kc, vc, eps,
+                              interleaved=False):
+        """qk_norm_rope_kv for a batch of tokens over a paged cache, every token at its own position (no counterpart in
+        the reference; lfm2q_qk_norm_rope_kv_paged has the rules): qkv bf16 or fp16 [N, (NQ + 2 NKV) * D] (the rows may
+        be strided), qw / kw [D] or both None, inv_freq fp32 [rot_dim / 2] (lfm2opt.rope), positions / slots int64 [N],
+        q_out [N, NQ, D], kc / vc [num_pages, NKV, page, D]."""
+        _req(qkv.is_cuda and qkv.dim() == 2 and qkv.stride(1) == 1, "qkv must be CUDA [N, (NQ + 2 NKV) * D], dense rows")
+        self._paged(qkv, kc, vc, "qkv")
+        for t, n in ((qw, "qw"), (kw, "kw"), (q_out, "q_out")):
+            _req(t is None and n != "q_out" or (t is not None and t.is_cuda and t.dtype == qkv.dtype
+                                                and t.is_contiguous()),
+                 f"{n} must be contiguous CUDA of qkv's dtype")
+        for t, n in ((positions, "positions"), (slots, "slots")):
+            _req(t.is_cuda and t.dtype == torch.int64 and t.is_contiguous(), f"{n} must be contiguous CUDA int64")
+        _check(inv_freq, _F32, "inv_freq")
+        N, (pages, NKV, page, D) = qkv.size(0), kc.shape
+        _req(q_out.dim() == 3 and q_out.size(0) == N and q_out.size(2) == D, "q_out [N, NQ, D]")
+        NQ = q_out.size(1)
+        _req(qkv.size(1) == (NQ + 2 * NKV) * D, "qkv [N, (NQ + 2 NKV) * D]")
+        _req(positions.numel() == N and slots.numel() == N, "positions, slots [N]")
+        _req((qw is None) == (kw is None), "qw and kw: both or neither")
+        _req(qw is None or (qw.numel() == D and kw.numel() == D), "qw, kw [D]")
+        self._same_device(qkv, qw, kw, inv_freq, positions, slots, q_out, kc, vc)
+        stride = qkv.stride(0) if N > 1 else qkv.size(1)
+        with _DeviceOf(qkv):
+            _capi.call("lfm2q_qk_norm_rope_kv_paged", qkv.data_ptr(), stride, _ptr(qw), _ptr(kw), inv_freq.data_ptr(),
+                       2 * inv_freq.numel(), float(scaling), positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(),
+                       kc.data_ptr(), vc.data_ptr(), _capi.BF16 if qkv.dtype == _BF else _capi.FP16, N, NQ, NKV, D,
+                       pages, page, float(eps), int(bool(interleaved)), _stream(qkv))
+
+    def tree_attention_splits(self, B, NQ, NKV, D, max_q, max_len):
+        """The number of splits that fills the current device for B requests of up to max_q drafted tokens and max_len
+        positions: the S of tree_attention's workspace."""
+        return _capi.lib().lfm2q_tree_attention_splits(int(B), int(NQ), int(NKV), int(D), int(max_q), int(max_len))
+
+    def tree_attention(self, q, kc, vc, table, ctx, cu, mask, out, ws, scale, max_q):
+        """Attention of drafted tokens over a paged cache (no counterpart in the reference; lfm2q_tree_attention has the
+        rules): q, out bf16 or fp16 [N, NQ, D], kc / vc [num_pages, NKV, page, D], table int32 [B, max_pages], ctx int32
+        [B], cu int32 [B + 1], mask int64 [N] (bit j: the token sees its request's draft j) or None (a chain), ws fp32
+        [N, NQ, S, D + 2] (S = tree_attention_splits(...)) or None (S = 1), max_q <= 64 the most tokens of a request."""
+        for t, n in ((q, "q"), (out, "out")):
+            _req(t.is_cuda and t.is_contiguous() and t.dim() == 3, f"{n} must be contiguous CUDA [N, NQ, D]")
+        self._paged(q, kc, vc, "q")
+        _req(out.dtype == q.dtype and out.shape == q.shape, "out must be like q")
+        N, NQ, D = q.shape
+        pages, NKV, page, _ = kc.shape
+        _req(kc.size(3) == D and NQ % NKV == 0, "q [N, NQ, D], kc / vc [num_pages, NKV, page, D], NQ a multiple of NKV")
+        for t, n in ((table, "table"), (ctx, "ctx"), (cu, "cu")):
+            _req(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous(), f"{n} must be contiguous CUDA int32")
+        B = ctx.numel()
+        _req(table.dim() == 2 and table.size(0) == B and cu.numel() == B + 1, "table [B, max_pages], cu [B + 1]")
+        _req(mask is None or (mask.is_cuda and mask.dtype == torch.int64 and mask.is_contiguous()
+                              and mask.numel() == N), "mask: contiguous CUDA int64 [N]")
+        _req(ws is None or (ws.is_cuda and ws.dtype == _F32 and ws.is_contiguous() and ws.dim() == 4
+                            and ws.shape[:2] == q.shape[:2] and ws.size(3) == D + 2), "ws: fp32 [N, NQ, S, D + 2]")
+        self._same_device(q, kc, vc, table, ctx, cu, mask, out, ws)
+        with _DeviceOf(q):
+            _capi.call("lfm2q_tree_attention", q.data_ptr(), kc.data_ptr(), vc.data_ptr(), table.data_ptr(),
+                       ctx.data_ptr(), cu.data_ptr(), _ptr(mask), out.data_ptr(), _ptr(ws),
+                       _capi.BF16 if q.dtype == _BF else _capi.FP16, N, B, NQ, NKV, D, pages, page, table.size(1),
+                       1 if ws is None else ws.size(2), int(max_q), float(scale), _stream(q))
+
+    def sample_next(self, logits, temperature, top_k, top_p, min_p, u, tok, pos=None):
+        """argmax_next's counterpart that samples (no counterpart in the reference; lfm2q_sample_next has the rules):
+        logits bf16, fp16 or fp32 [B, V] (the rows may be strided), temperature / top_p / min_p fp32 [B] and top_k
+        int32 [B], each or None, u fp32 [B] uniform in [0, 1), tok int64 [B] written; then pos[0] += 1 if given."""
+        dt = {_BF: _capi.BF16, torch.float16: _capi.FP16, _F32: _capi.FP32}.get(logits.dtype)
+        _req(logits.is_cuda and dt is not None and logits.dim() == 2 and logits.stride(1) == 1,
+             "logits must be CUDA bf16, fp16 or fp32 [B, V], dense rows")
+        B, V = logits.shape
+        for t, n in ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (u, "u")):
+            _req((t is None and n != "u") or (t is not None and t.is_cuda and t.dtype == _F32 and t.is_contiguous()
+                                              and t.numel() == B), f"{n}: contiguous CUDA fp32 [B]")
+        _req(top_k is None or (top_k.is_cuda and top_k.dtype == torch.int32 and top_k.is_contiguous()
+                               and top_k.numel() == B), "top_k: contiguous CUDA int32 [B]")
+        _req(tok.is_cuda and tok.dtype == torch.int64 and tok.is_contiguous() and tok.numel() == B,
+             "tok: contiguous CUDA int64 [B]")
+        _req(pos is None or (pos.is_cuda and pos.dtype == torch.int64), "pos: CUDA int64 [1]")
+        self._same_device(logits, temperature, top_k, top_p, min_p, u, tok, pos)
+        with _DeviceOf(logits):
+            _capi.call("lfm2q_sample_next", logits.data_ptr(), dt, logits.stride(0) if B > 1 else V,
+                       _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), u.data_ptr(), tok.data_ptr(),
+                       _ptr(pos), B, V, _stream(logits))
+
     def set_pdl(self, on):
         """Enable/disable Programmatic Dependent Launch for the GEMV kernels (default on)."""
         _capi.lib().lfm2q_set_pdl(int(bool(on)))

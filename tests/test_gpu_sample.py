@@ -1,0 +1,154 @@
+"""Sampling (sample_next) on the B200: whole numbers, equal to the definition in 64 bits.
+
+The kernel sums weights in steps of 2^-44 of the largest; on the fixed seeds here no draw falls within that of a border,
+so every token is equal.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from lfm2opt.kernels import ext
+from oracle.serving import sample_next_f64
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+
+
+def draw(dev, x, temperature=None, top_k=None, top_p=None, min_p=None, u=None, pos=None):
+    B = x.shape[0]
+    f = lambda a, t=torch.float32: None if a is None else torch.tensor(a, dtype=t, device=dev)  # noqa: E731
+    tok = torch.full((B,), -1, dtype=torch.int64, device=dev)
+    ext().sample_next(x.to(dev) if not x.is_cuda else x, f(temperature), f(top_k, torch.int32), f(top_p), f(min_p),
+                      f(u), tok, pos)
+    return tok.cpu().tolist()
+
+
+def want(x, temperature, top_k, top_p, min_p, u):
+    r = np.float32  # the kernel takes fp32 parameters
+    return [sample_next_f64(row.double().numpy(), float(r(t)), k, float(r(p)), float(r(m)), float(r(v)))
+            for row, t, k, p, m, v in zip(x.cpu(), temperature, top_k, top_p, min_p, u)]
+
+
+def params(rng, B):
+    pick = lambda *a: [a[i] for i in rng.integers(0, len(a), B)]  # noqa: E731
+    return dict(temperature=pick(0.0, 0.2, 0.7, 1.0, 3.0), top_k=pick(0, 0, 1, 2, 40, 1000, 10**6),
+                top_p=pick(1.0, 0.95, 0.9, 0.5, 0.01, 0.0), min_p=pick(0.0, 0.0, 0.05, 0.5, 1.0),
+                u=rng.random(B, dtype=np.float32).tolist())
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("V", [1, 2, 7, 8, 33, 1009, 4096, 50001, 65536])
+def test_equal_to_the_definition(cuda_dev, V, dt):
+    rng = np.random.default_rng(V)
+    B = 40 if V < 5000 else 16
+    g = torch.Generator().manual_seed(V)
+    x = (2.5 * torch.randn(B, V, generator=g) + 6 * (torch.rand(B, V, generator=g) < 20 / V)).to(DT[dt])
+    p = params(rng, B)
+    assert draw(cuda_dev, x, **p) == want(x, **p)
+
+
+@pytest.mark.parametrize("B", [1, 3, 200])
+def test_batch_sizes_and_strided_rows(cuda_dev, B):
+    """One row spread over a cluster, and a batch of one block a row; rows 2 bytes off any alignment."""
+    g = torch.Generator().manual_seed(B)
+    wide = (3 * torch.randn(B, 9003, generator=g)).bfloat16().to(cuda_dev)
+    x = wide[:, 1:9002]
+    p = params(np.random.default_rng(B), B)
+    assert draw(cuda_dev, x, **p) == want(x, **p)
+
+
+def test_largest_vocabulary(cuda_dev):
+    g = torch.Generator().manual_seed(3)
+    x = torch.randn(2, 1 << 18, generator=g) * 2
+    for dt in DT.values():
+        p = dict(temperature=[1.0, 0.9], top_k=[0, 5000], top_p=[0.97, 0.99], min_p=[0.0, 0.0], u=[0.83, 0.4])
+        assert draw(cuda_dev, x.to(dt), **p) == want(x.to(dt), **p)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+def test_ties_infinities_and_nans(cuda_dev, dt):
+    inf, nan = float("inf"), float("nan")
+    V = 3000
+    rows, p = [], dict(temperature=[], top_k=[], top_p=[], min_p=[], u=[])
+
+    def add(row, T=1.0, k=0, tp=1.0, mp=0.0, u=0.5):
+        rows.append(row)
+        for n, v in zip(p, (T, k, tp, mp, u)):
+            p[n].append(v)
+
+    flat = torch.zeros(V)
+    for u in (0.0, 0.1234, 0.999999):
+        add(flat, u=u)                      # all equal
+        add(flat, k=7, u=u)                 # ties at the cut: the lowest indexes
+        add(flat, tp=0.25, u=u)
+        add(flat, k=1000, tp=0.5, u=u)
+        add(flat, mp=1.0, u=u)
+    some = torch.full((V,), -inf)
+    some[[5, 99, 2000]] = torch.tensor([1.0, 2.0, 1.0])
+    for u in (0.0, 0.3, 0.99):
+        add(some, u=u)
+        add(some, k=2, u=u)                 # one of two equal ones: the lower index
+        add(some, k=500, tp=0.999, u=u)     # more asked for than there is mass
+    add(torch.full((V,), -inf))             # nothing finite: the first
+    top = flat.clone()
+    top[[17, 30]] = inf
+    add(top, u=0.2), add(top, u=0.7), add(top, k=1), add(top, T=0.0)
+    bad = flat.clone()
+    bad[40], bad[41] = nan, nan
+    add(bad), add(bad, T=0.0)
+    signs = torch.where(torch.arange(V) % 2 == 0, -0.0, 0.0)
+    add(signs, k=3, u=0.9), add(signs, k=3, u=0.1)  # zeros of both signs are one value
+    tiny = torch.zeros(V)
+    tiny[:4] = torch.tensor([1e-30, -1e-30, 2e-38, -2e-38])
+    add(tiny, k=2, u=0.9), add(tiny, k=4, u=0.9), add(tiny, tp=0.001, u=0.9)
+    spread = torch.linspace(-60000, 60000, V)
+    add(spread, T=1e-3, u=0.5), add(spread, T=1e6, tp=0.5, u=0.5), add(spread, T=1e30, u=0.7), add(spread, T=inf, u=0.7)
+    add(spread, T=nan), add(spread, tp=nan, T=30.0), add(spread, mp=nan, T=30.0), add(spread, T=-1.0)
+    add(spread, T=30.0, mp=7.0, u=0.9), add(spread, T=30.0, tp=-1.0, u=0.9), add(spread, T=30.0, k=-4, u=0.9)
+    x = torch.stack(rows).to(DT[dt])
+    assert draw(cuda_dev, x, **p) == want(x, **p)
+
+
+def test_off_switches_and_position(cuda_dev):
+    g = torch.Generator().manual_seed(1)
+    x = torch.randn(4, 500, generator=g)
+    u = [0.1, 0.4, 0.6, 0.9]
+    pos = torch.tensor([41], device=cuda_dev)
+    assert draw(cuda_dev, x, u=u, pos=pos) == want(x, [1.0] * 4, [0] * 4, [1.0] * 4, [0.0] * 4, u)
+    assert int(pos) == 42
+    tok = torch.empty(4, dtype=torch.int64, device=cuda_dev)
+    ext().argmax_next(x.bfloat16()[:, :496].contiguous().to(cuda_dev), tok)
+    assert draw(cuda_dev, x.bfloat16()[:, :496], temperature=[0.0] * 4, u=u) == tok.cpu().tolist()
+
+
+def test_distribution(cuda_dev):
+    """Evenly spaced uniforms give every token its share, to one draw."""
+    x = torch.tensor([[0.0, 1.0, 2.0, -1.0, 0.5]])
+    n = 4000
+    toks = draw(cuda_dev, x.expand(n, 5).contiguous(), u=((np.arange(n) + 0.5) / n).tolist())
+    share = torch.softmax(x[0].double(), 0) * n
+    for i in range(5):
+        assert abs(toks.count(i) - share[i].item()) <= 1.0
+
+
+def test_capture_and_refusals(cuda_dev):
+    g = torch.Generator().manual_seed(2)
+    x = torch.randn(3, 2000, generator=g).to(cuda_dev)
+    u, tok = torch.rand(3, device=cuda_dev), torch.zeros(3, dtype=torch.int64, device=cuda_dev)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ext().sample_next(x, None, None, None, None, u, tok)
+    x.copy_(torch.randn(3, 2000, generator=g).to(cuda_dev))
+    graph.replay()
+    assert tok.cpu().tolist() == want(x, [1.0] * 3, [0] * 3, [1.0] * 3, [0.0] * 3, u.cpu().tolist())
+    K = ext()
+    K.sample_next(x[:0], None, None, None, None, u[:0], tok[:0])
+    for args, match in (((x.double(), None, None, None, None, u, tok), "logits"),
+                        ((x.t(), None, None, None, None, u, tok), "logits"),
+                        ((x, u[:2], None, None, None, u, tok), "temperature"),
+                        ((x, None, u, None, None, u, tok), "top_k"), ((x, None, None, None, None, None, tok), "u:"),
+                        ((x, None, None, None, None, u, tok.int()), "tok"),
+                        ((torch.zeros(3, (1 << 18) + 1, device=cuda_dev), None, None, None, None, u, tok), "262144")):
+        with pytest.raises(RuntimeError, match=match):
+            K.sample_next(*args)

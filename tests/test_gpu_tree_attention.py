@@ -1,0 +1,227 @@
+"""Attention of drafted tokens over a paged cache (tree_attention) on the B200, against 64 bits.
+
+Tolerance, from the arithmetic: every probability is rounded once to the type (eps / 2 of it) before the second product
+while the sum keeps it unrounded, the output once more; fp32 sums and exponentials of up to some thousand terms add less
+than 2e-5 of the largest |v|. So |err| <= eps / 2 (|out| + sum_t p_t |v_t|) + 2e-5 max |v|, and sum p |v| <= max |v|:
+the bound used is eps / 2 (|out| + max |v|) + 2e-5 max |v|, max |v| over the request's values of that head.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+from lfm2opt.kernels import ext
+from oracle.serving import tree_attention_f64
+
+pytestmark = pytest.mark.gpu
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16}
+
+
+def make(seed, NQ, NKV, D, page, ctx, T, dt, chain=False, spare=2, pad_rows=0, width=None):
+    """CPU tensors of a batch: random trees (masks as Python ints), pages in random order."""
+    rng = np.random.default_rng(seed)
+    g = torch.Generator().manual_seed(seed)
+    used = [-(-(c + t) // page) for c, t in zip(ctx, T)]
+    pages = sum(used) + spare
+    ids = rng.permutation(pages)
+    table = np.full((len(ctx), width or max(max(used), 1)), -1, np.int32)
+    at, masks = 0, []
+    for b, n in enumerate(used):
+        table[b, :n] = ids[at:at + n]
+        at += n
+        m = []
+        for i in range(T[b]):
+            up = 0 if i == 0 else m[i - 1 if chain else int(rng.integers(max(0, i - 4), i))]
+            m.append(up | (1 << i))
+        masks += m
+    N = sum(T) + pad_rows
+    masks += [0] * pad_rows
+    cu = np.concatenate([[0], np.cumsum(T)]).astype(np.int32)
+    rn = lambda *s: torch.randn(*s, generator=g).to(DT[dt])  # noqa: E731
+    return dict(q=rn(N, NQ, D), kc=rn(pages, NKV, page, D), vc=rn(pages, NKV, page, D),
+                table=torch.from_numpy(table), ctx=torch.tensor(ctx, dtype=torch.int32), cu=torch.from_numpy(cu),
+                mask=None if chain else masks, scale=D ** -0.5, max_q=max(max(T), 1))
+
+
+def signed(masks):
+    return torch.tensor([m - (1 << 64) if m >> 63 else m for m in masks], dtype=torch.int64)
+
+
+def run(dev, c, S=None):
+    N, NQ, D = c["q"].shape
+    d = {k: v.to(dev) for k, v in c.items() if torch.is_tensor(v)}
+    out = torch.full(c["q"].shape, float("nan"), dtype=c["q"].dtype, device=dev)
+    if S is None:
+        S = ext().tree_attention_splits(len(c["ctx"]), NQ, c["kc"].shape[1], D, c["max_q"],
+                                        c["table"].shape[1] * c["kc"].shape[2])
+    ws = torch.full((N, NQ, S, D + 2), float("nan"), device=dev) if S > 1 else None
+    ext().tree_attention(d["q"], d["kc"], d["vc"], d["table"], d["ctx"], d["cu"],
+                         None if c["mask"] is None else signed(c["mask"]).to(dev), out, ws, c["scale"], c["max_q"])
+    torch.cuda.synchronize()
+    return out
+
+
+def reference(c):
+    return tree_attention_f64(c["q"], c["kc"], c["vc"], c["table"], c["ctx"], c["cu"], c["mask"], c["scale"],
+                              c["max_q"])
+
+
+def check(out, ref, c):
+    vmax = c["vc"].float()
+    vmax = vmax[vmax.isfinite()].abs().max().item()
+    out = out.cpu().double()
+    assert torch.equal(out.isnan(), ref.isnan())  # rows outside the requests: as they were
+    err, lim = (out - ref).abs(), torch.finfo(c["q"].dtype).eps / 2 * (ref.abs() + vmax) + 2e-5 * vmax
+    ok = ref.isnan() | (err <= lim)
+    assert ok.all(), (err[~ok].max().item(), (~ok).nonzero()[:4].tolist())
+
+
+CASES = [
+    # NQ, NKV, D, page, ctx, T, dt, chain
+    (32, 8, 64, 64, [1000], [1], "bf16", True),
+    (4, 1, 64, 16, [0], [1], "fp16", True),
+    (8, 8, 64, 1, [5, 0, 17], [1, 2, 3], "bf16", False),
+    (32, 8, 64, 64, [0, 63, 64, 200], [8, 8, 7, 1], "bf16", False),
+    (24, 3, 128, 16, [0, 100, 777], [13, 2, 4], "fp16", False),
+    (16, 2, 128, 24, [300, 50], [16, 9], "bf16", False),
+    (6, 2, 64, 7, [129, 1], [64, 33], "fp16", False),
+    (8, 1, 128, 128, [400], [64], "bf16", True),
+    (64, 1, 64, 32, [90], [5], "bf16", False),
+    (12, 4, 128, 64, [0, 0], [0, 21], "fp16", False),
+]
+
+
+@pytest.mark.parametrize("S", [None, 1, 3])
+@pytest.mark.parametrize("NQ,NKV,D,page,ctx,T,dt,chain", CASES)
+def test_tree_attention_against_64_bits(cuda_dev, NQ, NKV, D, page, ctx, T, dt, chain, S):
+    c = make(len(ctx) + NQ + page, NQ, NKV, D, page, ctx, T, dt, chain, pad_rows=3)
+    check(run(cuda_dev, c, S), reference(c), c)
+
+
+@pytest.mark.parametrize("max_ctx,B,T", [(2500, 3, 16), (2500, 1, 1), (2000, 2, 64)])
+def test_longer_contexts(cuda_dev, max_ctx, B, T):
+    c = make(B, 8, 2, 64, 16, [max_ctx - 700 * b for b in range(B)], [T] * B, "bf16")
+    check(run(cuda_dev, c), reference(c), c)
+
+
+def test_queries_that_see_nothing_give_zeros(cuda_dev):
+    c = make(1, 8, 2, 64, 16, [0, 0, 40], [5, 1, 3], "bf16")
+    c["mask"] = [0, 1, 0, 12, 0, 0, 0, 7, 0]
+    out, ref = run(cuda_dev, c), reference(c)
+    check(out, ref, c)
+    assert torch.count_nonzero(out[[0, 2, 4, 5]]) == 0
+
+
+def test_masked_infinities_and_nans_do_not_spread(cuda_dev):
+    """Drafts that hold an infinity or a NaN reach the queries that see them and no others; stale rows behind the
+    length and unused pages are never read into a result."""
+    for D, dt, T in ((64, "bf16", 7), (128, "fp16", 20), (64, "fp16", 64)):
+        c = make(3, 8, 2, D, 16, [70, 33], [T, 5], dt, spare=2)
+        k, v = c["kc"], c["vc"]
+        live = torch.zeros(k.shape[0], 16, dtype=torch.bool)
+        for b, L in enumerate((70 + T, 38)):
+            for t in range(L):
+                live[c["table"][b, t // 16], t % 16] = True
+        k.transpose(1, 2)[~live] = float("nan")
+        v.transpose(1, 2)[~live] = float("inf")
+        poison = 70 + 3  # draft 3 of request 0
+        pg, r = int(c["table"][0, poison // 16]), poison % 16
+        v[pg, 0, r, 5], v[pg, 1, r, D - 1], k[pg, 0, r, 2] = float("inf"), float("nan"), float("nan")
+        sees = [bool((m >> 3) & 1) for m in c["mask"][:T]]
+        clean = dict(c, kc=k.clone(), vc=v.clone())
+        clean["kc"].nan_to_num_(0, 0, 0), clean["vc"].nan_to_num_(0, 0, 0)
+        for S in (1, 2):
+            out, ref = run(cuda_dev, c, S), reference(clean)
+            blind = [i for i in range(T) if not sees[i]] + list(range(T, T + 5))
+            check(out[blind], ref[blind], clean)
+            seeing = [i for i in range(T) if sees[i]]
+            assert not out[seeing, :4].isfinite().all(-1).any() and out[seeing, 4:, D - 1].isnan().all()
+
+
+def test_pages_outside_the_pool_are_not_seen(cuda_dev):
+    c = make(4, 8, 2, 64, 16, [100, 30], [4, 4], "bf16")
+    c["table"][0, 2], c["table"][1, 0] = -1, c["kc"].shape[0]
+    check(run(cuda_dev, c, 2), reference(c), c)
+    c["ctx"][1] = 100000  # past the table: what the table holds
+    check(run(cuda_dev, c), reference(c), c)
+
+
+def test_more_queries_than_max_q_are_left(cuda_dev):
+    c = make(5, 4, 1, 64, 16, [20], [9], "bf16")
+    c["max_q"] = 6
+    out = run(cuda_dev, c)
+    assert out[6:].isnan().all()
+    ref = tree_attention_f64(c["q"], c["kc"], c["vc"], c["table"], c["ctx"], c["cu"], c["mask"], c["scale"], 6)
+    check(out, ref, c)
+
+
+def test_dense_cache_is_one_page_per_request(cuda_dev):
+    """page = max_len and table[b] = {b}: the cache of decode_attention_split, and its result."""
+    g = torch.Generator().manual_seed(9)
+    B, NKV, L, pos = 3, 8, 777, 500
+    q = torch.randn(B, 32, 64, generator=g).bfloat16().to(cuda_dev)
+    kc, vc = [torch.randn(B, NKV, L, 64, generator=g).bfloat16().to(cuda_dev) for _ in range(2)]
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=cuda_dev)  # noqa: E731
+    a, b = torch.empty_like(q), torch.empty_like(q)
+    ext().decode_attention_split(q, kc, vc, torch.tensor([pos], device=cuda_dev), a,
+                                 torch.empty(B, 32, 4, 66, device=cuda_dev), 0.125)
+    ext().tree_attention(q, kc, vc, i32([[0], [1], [2]]), i32([pos] * B), i32([0, 1, 2, 3]), None, b, None, 0.125, 1)
+    # two roundings of the output and one of every probability
+    lim = torch.finfo(q.dtype).eps / 2 * (2 * a.float().abs() + vc.float().abs().max()) + 4e-5 * vc.float().abs().max()
+    assert ((a.float() - b.float()).abs() <= lim).all()
+
+
+def test_repeatable_and_capturable(cuda_dev):
+    c = make(6, 32, 8, 64, 64, [900, 64], [16, 3], "bf16")
+    first = run(cuda_dev, c)
+    assert torch.equal(first.nan_to_num(), run(cuda_dev, c).nan_to_num())
+    d = {k: v.to(cuda_dev) for k, v in c.items() if torch.is_tensor(v)}
+    mask, out = signed(c["mask"]).to(cuda_dev), torch.full_like(first, float("nan"))
+    S = ext().tree_attention_splits(2, 32, 8, 64, 16, 1024)
+    ws = torch.empty(19, 32, S, 66, device=cuda_dev) if S > 1 else None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ext().tree_attention(d["q"], d["kc"], d["vc"], d["table"], d["ctx"], d["cu"], mask, out, ws, c["scale"], 16)
+    d["q"].zero_()
+    graph.replay()  # uniform attention over what is seen
+    torch.cuda.synchronize()
+    zero = dict(c, q=torch.zeros_like(c["q"]))
+    check(out, reference(zero), zero)
+
+
+def test_long_cache_offsets_pass_32_bits(cuda_dev):
+    """A pool whose last page starts behind 2^32 elements: the request sits at its far end."""
+    NKV, page, D = 8, 64, 64
+    pages = (1 << 32) // (NKV * page * D) + 5  # 8.6 GB a cache
+    kc = torch.zeros(pages, NKV, page, D, dtype=torch.bfloat16, device=cuda_dev)
+    vc = torch.zeros_like(kc)
+    c = make(8, 32, NKV, D, page, [150], [3], "bf16", spare=0)
+    ids = torch.tensor([pages - 1, 0, pages - 3])
+    kc[ids.to(cuda_dev)], vc[ids.to(cuda_dev)] = c["kc"][c["table"][0].long()].to(cuda_dev), \
+        c["vc"][c["table"][0].long()].to(cuda_dev)
+    q = c["q"].to(cuda_dev)
+    out = torch.full_like(q, float("nan"))
+    i32 = lambda t: t.to(torch.int32).to(cuda_dev)  # noqa: E731
+    ext().tree_attention(q, kc, vc, i32(ids)[None], i32(c["ctx"]), i32(c["cu"]), signed(c["mask"]).to(cuda_dev), out,
+                         None, c["scale"], 3)
+    check(out, reference(c), c)
+
+
+def test_refusals(cuda_dev):
+    c = make(7, 8, 2, 64, 16, [20], [3], "bf16")
+    d = {k: v.to(cuda_dev) for k, v in c.items() if torch.is_tensor(v)}
+    out, m = torch.empty_like(d["q"]), signed(c["mask"]).to(cuda_dev)
+
+    def call(**kw):
+        a = dict(d, mask=m, out=out, ws=None, scale=0.125, max_q=3, **{})
+        a.update(kw)
+        ext().tree_attention(a["q"], a["kc"], a["vc"], a["table"], a["ctx"], a["cu"], a["mask"], a["out"], a["ws"],
+                             a["scale"], a["max_q"])
+
+    for kw, match in ((dict(max_q=65), "max_q"), (dict(max_q=0), "max_q"), (dict(scale=0.0), "scale"),
+                      (dict(q=d["q"].float(), out=out.float()), "bf16 or fp16"), (dict(mask=m[:2]), "mask"),
+                      (dict(kc=d["kc"].half()), "dtype"), (dict(cu=d["cu"][:1]), "cu"),
+                      (dict(table=d["table"].long()), "int32"), (dict(q=d["q"][:, :3]), "contiguous"),
+                      (dict(ws=torch.empty(3, 8, 2, 64, device=cuda_dev)), "ws")):
+        with pytest.raises(RuntimeError, match=match):
+            call(**kw)
