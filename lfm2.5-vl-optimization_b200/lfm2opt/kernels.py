@@ -31,6 +31,33 @@ def _check(t, dtype, name):
 _DT_NAME = {_I8: "at::kChar", _BF: "at::kBFloat16", _F32: "at::kFloat"}
 
 
+_I32, _I64 = torch.int32, torch.int64
+_HALF = {torch.bfloat16: _capi.BF16, torch.float16: _capi.FP16}
+_FLOAT = {**_HALF, torch.float32: _capi.FP32}
+
+
+def _arg(t, dtype, name, dev):
+    """The device pointer of t, checked: a dense tensor of dtype on device dev."""
+    if not (t.is_cuda and t.dtype is dtype and t.is_contiguous()):
+        raise RuntimeError(f"{name} must be contiguous CUDA, dtype {dtype}")
+    if t.get_device() != dev:
+        raise RuntimeError(f"{name}: every tensor must be on one device")
+    return t.data_ptr()
+
+
+def _launch(fn, dev, *args):
+    """Call entry point fn(*args, stream) on PyTorch's current stream of device dev, that device current; raise
+    RuntimeError with the library's message on a non-OK status."""
+    prev = torch._C._cuda_getDevice()
+    if prev != dev:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if st != _capi.OK:
+        raise RuntimeError(_capi.lib().lfm2q_last_error().decode() or f"lfm2q: status {st}")
+
+
 def _req(cond, msg):
     if not cond:
         raise RuntimeError(msg)
@@ -412,40 +439,36 @@ class DecodeGemvExt:
                        out.data_ptr(), ws.data_ptr(), B, NQ, NKV, max_len, ws.size(2), float(scale), _stream(q))
 
     # -------------------------------------------------- batches of requests over a paged cache (include/lfm2q.h)
-    @staticmethod
-    def _same_device(first, *rest):
-        for t in rest:
-            _req(t is None or t.device == first.device, "every tensor must be on one device")
-
+    # These are called a few times a decode iteration on small work, so the checks are written to cost little on the
+    # host: one helper call a tensor that returns its pointer, messages formed only on failure (16-20 us a call with
+    # the checks above, 8-10 us so).
     def kv_slots(self, lens, new_lens, table, free, n_free, page, got, cu, positions, slots):
         """Block tables and slot maps from request lengths (no counterpart in the reference; lfm2q_kv_slots has the
         rules). lens, new_lens, got int32 [B], table int32 [B, max_pages], free int32 [num_pages] with n_free int32 [1]
         entries (a stack), cu int32 [B + 1], positions / slots int64 [capacity]: table, free and n_free are updated in
         place; got, cu and the first cu[B] rows of positions and slots are written."""
-        for t, n in ((lens, "lens"), (new_lens, "new_lens"), (table, "table"), (free, "free"), (n_free, "n_free"),
-                     (got, "got"), (cu, "cu")):
-            _req(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous(), f"{n} must be contiguous CUDA int32")
-        for t, n in ((positions, "positions"), (slots, "slots")):
-            _req(t.is_cuda and t.dtype == torch.int64 and t.is_contiguous(), f"{n} must be contiguous CUDA int64")
-        B = lens.numel()
-        _req(table.dim() == 2 and table.size(0) == B and table.size(1) > 0, "table [B, max_pages]")
-        _req(new_lens.numel() == B and got.numel() == B and cu.numel() == B + 1 and n_free.numel() == 1,
-             "lens, new_lens, got [B], cu [B + 1], n_free [1]")
-        _req(positions.numel() == slots.numel(), "positions and slots: one length")
-        self._same_device(lens, new_lens, table, free, n_free, got, cu, positions, slots)
-        with _DeviceOf(lens):
-            _capi.call("lfm2q_kv_slots", lens.data_ptr(), new_lens.data_ptr(), table.data_ptr(), free.data_ptr(),
-                       n_free.data_ptr(), got.data_ptr(), cu.data_ptr(), positions.data_ptr(), slots.data_ptr(), B,
-                       table.size(1), free.numel(), int(page), slots.numel(), _stream(lens))
+        dev, B, capacity = lens.get_device(), lens.numel(), slots.numel()
+        p = (_arg(lens, _I32, "lens", dev), _arg(new_lens, _I32, "new_lens", dev), _arg(table, _I32, "table", dev),
+             _arg(free, _I32, "free", dev), _arg(n_free, _I32, "n_free", dev), _arg(got, _I32, "got", dev),
+             _arg(cu, _I32, "cu", dev), _arg(positions, _I64, "positions", dev), _arg(slots, _I64, "slots", dev))
+        if table.dim() != 2 or table.size(0) != B or table.size(1) == 0:
+            raise RuntimeError("table must be [B, max_pages]")
+        if not (new_lens.numel() == B == got.numel() and cu.numel() == B + 1 and n_free.numel() == 1):
+            raise RuntimeError("need lens, new_lens, got [B], cu [B + 1], n_free [1]")
+        if positions.numel() != capacity:
+            raise RuntimeError("positions and slots must have one length")
+        _launch(_capi.lib().lfm2q_kv_slots, dev, *p, B, table.size(1), free.numel(), page, capacity)
 
     @staticmethod
-    def _paged(q, kc, vc, name):
-        _req(q.dtype in (_BF, torch.float16), f"{name} must be bf16 or fp16")
-        for t, n in ((kc, "kc"), (vc, "vc")):
-            _req(t.is_cuda and t.dtype == q.dtype and t.is_contiguous() and t.dim() == 4,
-                 f"{n} must be contiguous CUDA [num_pages, NKV, page, D] of {name}'s dtype")
-        _req(vc.shape == kc.shape, "kc and vc: one shape")
-        _req(kc.size(3) in (64, 128), "head_dim 64 or 128 only")
+    def _paged(dtype, kc, vc, name, dev):
+        """(lfm2q dtype, kc and vc pointers, their shape)"""
+        dt = _HALF.get(dtype)
+        if dt is None:
+            raise RuntimeError(f"{name} must be bf16 or fp16")
+        shape = kc.shape
+        if len(shape) != 4 or vc.shape != shape or shape[3] not in (64, 128):
+            raise RuntimeError("kc and vc must be [num_pages, NKV, page, head_dim], head_dim 64 or 128 only")
+        return dt, _arg(kc, dtype, "kc", dev), _arg(vc, dtype, "vc", dev), shape
 
     def qk_norm_rope_kv_paged(self, qkv, qw, kw, inv_freq, scaling, positions, slots, q_out, kc, vc, eps,
                               interleaved=False):
@@ -453,29 +476,30 @@ class DecodeGemvExt:
         the reference; lfm2q_qk_norm_rope_kv_paged has the rules): qkv bf16 or fp16 [N, (NQ + 2 NKV) * D] (the rows may
         be strided), qw / kw [D] or both None, inv_freq fp32 [rot_dim / 2] (lfm2opt.rope), positions / slots int64 [N],
         q_out [N, NQ, D], kc / vc [num_pages, NKV, page, D]."""
-        _req(qkv.is_cuda and qkv.dim() == 2 and qkv.stride(1) == 1, "qkv must be CUDA [N, (NQ + 2 NKV) * D], dense rows")
-        self._paged(qkv, kc, vc, "qkv")
-        for t, n in ((qw, "qw"), (kw, "kw"), (q_out, "q_out")):
-            _req(t is None and n != "q_out" or (t is not None and t.is_cuda and t.dtype == qkv.dtype
-                                                and t.is_contiguous()),
-                 f"{n} must be contiguous CUDA of qkv's dtype")
-        for t, n in ((positions, "positions"), (slots, "slots")):
-            _req(t.is_cuda and t.dtype == torch.int64 and t.is_contiguous(), f"{n} must be contiguous CUDA int64")
-        _check(inv_freq, _F32, "inv_freq")
-        N, (pages, NKV, page, D) = qkv.size(0), kc.shape
-        _req(q_out.dim() == 3 and q_out.size(0) == N and q_out.size(2) == D, "q_out [N, NQ, D]")
+        dev, dtype = qkv.get_device(), qkv.dtype
+        if not (qkv.is_cuda and qkv.dim() == 2 and qkv.stride(1) == 1):
+            raise RuntimeError("qkv must be CUDA [N, (NQ + 2 NKV) * D] with dense rows")
+        dt, kp, vp, (pages, NKV, page, D) = self._paged(dtype, kc, vc, "qkv", dev)
+        qp = _arg(q_out, dtype, "q_out", dev)
+        N, width = qkv.shape
+        if q_out.dim() != 3 or q_out.size(0) != N or q_out.size(2) != D:
+            raise RuntimeError("q_out must be [N, NQ, D]")
         NQ = q_out.size(1)
-        _req(qkv.size(1) == (NQ + 2 * NKV) * D, "qkv [N, (NQ + 2 NKV) * D]")
-        _req(positions.numel() == N and slots.numel() == N, "positions, slots [N]")
-        _req((qw is None) == (kw is None), "qw and kw: both or neither")
-        _req(qw is None or (qw.numel() == D and kw.numel() == D), "qw, kw [D]")
-        self._same_device(qkv, qw, kw, inv_freq, positions, slots, q_out, kc, vc)
-        stride = qkv.stride(0) if N > 1 else qkv.size(1)
-        with _DeviceOf(qkv):
-            _capi.call("lfm2q_qk_norm_rope_kv_paged", qkv.data_ptr(), stride, _ptr(qw), _ptr(kw), inv_freq.data_ptr(),
-                       2 * inv_freq.numel(), float(scaling), positions.data_ptr(), slots.data_ptr(), q_out.data_ptr(),
-                       kc.data_ptr(), vc.data_ptr(), _capi.BF16 if qkv.dtype == _BF else _capi.FP16, N, NQ, NKV, D,
-                       pages, page, float(eps), int(bool(interleaved)), _stream(qkv))
+        if width != (NQ + 2 * NKV) * D:
+            raise RuntimeError("qkv must be [N, (NQ + 2 NKV) * D]")
+        if (qw is None) != (kw is None):
+            raise RuntimeError("qw and kw: both or neither")
+        wq = wk = None
+        if qw is not None:
+            wq, wk = _arg(qw, dtype, "qw", dev), _arg(kw, dtype, "kw", dev)
+            if qw.numel() != D or kw.numel() != D:
+                raise RuntimeError("qw and kw must be [D]")
+        if positions.numel() != N or slots.numel() != N:
+            raise RuntimeError("positions and slots must be [N]")
+        _launch(_capi.lib().lfm2q_qk_norm_rope_kv_paged, dev, qkv.data_ptr(), qkv.stride(0) if N > 1 else width, wq,
+                wk, _arg(inv_freq, _F32, "inv_freq", dev), 2 * inv_freq.numel(), scaling,
+                _arg(positions, _I64, "positions", dev), _arg(slots, _I64, "slots", dev), qp, kp, vp, dt, N, NQ, NKV, D,
+                pages, page, eps, 1 if interleaved else 0)
 
     def tree_attention_splits(self, B, NQ, NKV, D, max_q, max_len):
         """The number of splits that fills the current device for B requests of up to max_q drafted tokens and max_len
@@ -487,49 +511,51 @@ class DecodeGemvExt:
         rules): q, out bf16 or fp16 [N, NQ, D], kc / vc [num_pages, NKV, page, D], table int32 [B, max_pages], ctx int32
         [B], cu int32 [B + 1], mask int64 [N] (bit j: the token sees its request's draft j) or None (a chain), ws fp32
         [N, NQ, S, D + 2] (S = tree_attention_splits(...)) or None (S = 1), max_q <= 64 the most tokens of a request."""
-        for t, n in ((q, "q"), (out, "out")):
-            _req(t.is_cuda and t.is_contiguous() and t.dim() == 3, f"{n} must be contiguous CUDA [N, NQ, D]")
-        self._paged(q, kc, vc, "q")
-        _req(out.dtype == q.dtype and out.shape == q.shape, "out must be like q")
-        N, NQ, D = q.shape
-        pages, NKV, page, _ = kc.shape
-        _req(kc.size(3) == D and NQ % NKV == 0, "q [N, NQ, D], kc / vc [num_pages, NKV, page, D], NQ a multiple of NKV")
-        for t, n in ((table, "table"), (ctx, "ctx"), (cu, "cu")):
-            _req(t.is_cuda and t.dtype == torch.int32 and t.is_contiguous(), f"{n} must be contiguous CUDA int32")
-        B = ctx.numel()
-        _req(table.dim() == 2 and table.size(0) == B and cu.numel() == B + 1, "table [B, max_pages], cu [B + 1]")
-        _req(mask is None or (mask.is_cuda and mask.dtype == torch.int64 and mask.is_contiguous()
-                              and mask.numel() == N), "mask: contiguous CUDA int64 [N]")
-        _req(ws is None or (ws.is_cuda and ws.dtype == _F32 and ws.is_contiguous() and ws.dim() == 4
-                            and ws.shape[:2] == q.shape[:2] and ws.size(3) == D + 2), "ws: fp32 [N, NQ, S, D + 2]")
-        self._same_device(q, kc, vc, table, ctx, cu, mask, out, ws)
-        with _DeviceOf(q):
-            _capi.call("lfm2q_tree_attention", q.data_ptr(), kc.data_ptr(), vc.data_ptr(), table.data_ptr(),
-                       ctx.data_ptr(), cu.data_ptr(), _ptr(mask), out.data_ptr(), _ptr(ws),
-                       _capi.BF16 if q.dtype == _BF else _capi.FP16, N, B, NQ, NKV, D, pages, page, table.size(1),
-                       1 if ws is None else ws.size(2), int(max_q), float(scale), _stream(q))
+        dev, dtype, B = q.get_device(), q.dtype, ctx.numel()
+        dt, kp, vp, (pages, NKV, page, D) = self._paged(dtype, kc, vc, "q", dev)
+        qp, op = _arg(q, dtype, "q", dev), _arg(out, dtype, "out", dev)
+        shape = q.shape
+        if len(shape) != 3 or out.shape != shape or shape[2] != D or shape[1] % NKV:
+            raise RuntimeError("q and out must be [N, NQ, D], D as in the cache and NQ a multiple of NKV")
+        N, NQ, _ = shape
+        if table.dim() != 2 or table.size(0) != B or cu.numel() != B + 1:
+            raise RuntimeError("table must be [B, max_pages] and cu [B + 1]")
+        mp = wp = None
+        S = 1
+        if mask is not None:
+            mp = _arg(mask, _I64, "mask", dev)
+            if mask.numel() != N:
+                raise RuntimeError("mask must be [N]")
+        if ws is not None:
+            wp = _arg(ws, _F32, "ws", dev)
+            if ws.dim() != 4 or ws.size(0) != N or ws.size(1) != NQ or ws.size(3) != D + 2:
+                raise RuntimeError("ws must be [N, NQ, S, D + 2]")
+            S = ws.size(2)
+        _launch(_capi.lib().lfm2q_tree_attention, dev, qp, kp, vp, _arg(table, _I32, "table", dev),
+                _arg(ctx, _I32, "ctx", dev), _arg(cu, _I32, "cu", dev), mp, op, wp, dt, N, B, NQ, NKV, D, pages, page,
+                table.size(1), S, max_q, scale)
 
     def sample_next(self, logits, temperature, top_k, top_p, min_p, u, tok, pos=None):
         """argmax_next's counterpart that samples (no counterpart in the reference; lfm2q_sample_next has the rules):
         logits bf16, fp16 or fp32 [B, V] (the rows may be strided), temperature / top_p / min_p fp32 [B] and top_k
         int32 [B], each or None, u fp32 [B] uniform in [0, 1), tok int64 [B] written; then pos[0] += 1 if given."""
-        dt = {_BF: _capi.BF16, torch.float16: _capi.FP16, _F32: _capi.FP32}.get(logits.dtype)
-        _req(logits.is_cuda and dt is not None and logits.dim() == 2 and logits.stride(1) == 1,
-             "logits must be CUDA bf16, fp16 or fp32 [B, V], dense rows")
+        dev, dt = logits.get_device(), _FLOAT.get(logits.dtype)
+        if not (logits.is_cuda and dt is not None and logits.dim() == 2 and logits.stride(1) == 1):
+            raise RuntimeError("logits must be CUDA bf16, fp16 or fp32 [B, V] with dense rows")
         B, V = logits.shape
-        for t, n in ((temperature, "temperature"), (top_p, "top_p"), (min_p, "min_p"), (u, "u")):
-            _req((t is None and n != "u") or (t is not None and t.is_cuda and t.dtype == _F32 and t.is_contiguous()
-                                              and t.numel() == B), f"{n}: contiguous CUDA fp32 [B]")
-        _req(top_k is None or (top_k.is_cuda and top_k.dtype == torch.int32 and top_k.is_contiguous()
-                               and top_k.numel() == B), "top_k: contiguous CUDA int32 [B]")
-        _req(tok.is_cuda and tok.dtype == torch.int64 and tok.is_contiguous() and tok.numel() == B,
-             "tok: contiguous CUDA int64 [B]")
-        _req(pos is None or (pos.is_cuda and pos.dtype == torch.int64), "pos: CUDA int64 [1]")
-        self._same_device(logits, temperature, top_k, top_p, min_p, u, tok, pos)
-        with _DeviceOf(logits):
-            _capi.call("lfm2q_sample_next", logits.data_ptr(), dt, logits.stride(0) if B > 1 else V,
-                       _ptr(temperature), _ptr(top_k), _ptr(top_p), _ptr(min_p), u.data_ptr(), tok.data_ptr(),
-                       _ptr(pos), B, V, _stream(logits))
+        p = []
+        for t, dtype, name in ((temperature, _F32, "temperature"), (top_k, _I32, "top_k"), (top_p, _F32, "top_p"),
+                               (min_p, _F32, "min_p")):
+            p.append(None if t is None else _arg(t, dtype, name, dev))
+            if t is not None and t.numel() != B:
+                raise RuntimeError(f"{name} must be [B]")
+        if u is None or u.numel() != B:
+            raise RuntimeError("u: one uniform a row, fp32 [B]")
+        if tok.numel() != B:
+            raise RuntimeError("tok must be [B]")
+        _launch(_capi.lib().lfm2q_sample_next, dev, logits.data_ptr(), dt, logits.stride(0) if B > 1 else V, *p,
+                _arg(u, _F32, "u", dev), _arg(tok, _I64, "tok", dev),
+                None if pos is None else _arg(pos, _I64, "pos", dev), B, V)
 
     def set_pdl(self, on):
         """Enable/disable Programmatic Dependent Launch for the GEMV kernels (default on)."""
