@@ -92,8 +92,10 @@ int lfm2q_check_device(int clear) {
   if (int e = device_gate()) return e;
   const int v = gemm_device_error(clear != 0);
   const int a = attn_device_error(clear != 0);
+  const int t = tree_device_error(clear != 0);
   if (v) return fail(LFM2Q_ETIMEOUT, "lfm2q: a GEMM pipeline wait timed out on the device");
   if (a) return fail(LFM2Q_ETIMEOUT, "lfm2q: a decode-attention stage wait timed out on the device");
+  if (t) return fail(LFM2Q_ETIMEOUT, "lfm2q: a tree-attention pipeline wait timed out on the device");
   return LFM2Q_OK;
 }
 
@@ -477,7 +479,8 @@ int lfm2q_tree_attention(const uint16_t *q, const uint16_t *kc, const uint16_t *
   REQUIRE(NQ > 0 && NQ % NKV == 0 && NQ / NKV <= 64, "NQ must be a multiple of NKV, at most 64 times it");
   REQUIRE(max_q >= 1 && max_q <= 64, "max_q (drafted tokens of a request) must be in [1, 64]");
   REQUIRE((long long)max_pages * page <= (1ll << 30), "max_pages * page must be <= 2^30");
-  REQUIRE(B <= 65535 && (long long)B * NKV <= 0x7fffffffLL, "B must be <= 65535");
+  REQUIRE(B <= 65535 && (long long)B * NKV * max_q <= 0x7fffffffLL, "B must be <= 65535 and B * NKV * max_q < 2^31");
+  REQUIRE((long long)num_pages * NKV <= 0x7fffffffLL, "num_pages * NKV must be < 2^31");
   REQUIRE(S >= 1 && S <= 65535, "ws [N, NQ, S, D + 2]: need 1 <= S <= 65535");
   REQUIRE(scale > 0.f && scale < 1e30f, "scale must be positive and finite");
   if (N == 0 || B == 0) return LFM2Q_OK;

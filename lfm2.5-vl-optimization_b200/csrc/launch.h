@@ -110,6 +110,7 @@ cudaError_t launch_qk_norm_rope_kv_paged(const void *qkv, long long row_stride, 
                                          bool pdl, cudaStream_t st);
 
 // tree_attention.cu: drafted tokens over the paged cache (half: fp16, else bf16); ws is read and written where S > 1
+int tree_device_error(bool clear);  // sticky code written by a bounded wait that gave up (0 = none)
 int tree_attention_splits(int B, int NQ, int NKV, int D, int max_q, long long max_len);
 cudaError_t launch_tree_attention(const void *q, const void *kc, const void *vc, const int *table, const int *ctx,
                                   const int *cu, const int64_t *mask, void *out, float *ws, int N, int B, int NQ,

@@ -24,11 +24,10 @@
 
 #include "common.cuh"
 #include "launch.h"
+#include "tree_attention.cuh"
 
 namespace lfm2q {
 namespace {
-
-constexpr int TA_KEYS = 64;  // keys per tile
 
 template <class T>
 struct Mma;
@@ -40,11 +39,6 @@ struct Mma<bf16> {
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) { return pack_bf16x2(lo, hi); }
-  static __device__ __forceinline__ float2 up2(uint32_t u) { return make_float2(bf_lo(u), bf_hi(u)); }
-  static __device__ __forceinline__ bool finite2(uint32_t u) {
-    return (u & 0x7f80u) != 0x7f80u && (u & 0x7f800000u) != 0x7f800000u;
-  }
 };
 template <>
 struct Mma<__half> {
@@ -53,14 +47,6 @@ struct Mma<__half> {
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-  }
-  static __device__ __forceinline__ uint32_t pack(float lo, float hi) {
-    const __half2 h = __floats2half2_rn(lo, hi);
-    return *reinterpret_cast<const uint32_t *>(&h);
-  }
-  static __device__ __forceinline__ float2 up2(uint32_t u) { return __half22float2(*reinterpret_cast<__half2 *>(&u)); }
-  static __device__ __forceinline__ bool finite2(uint32_t u) {
-    return (u & 0x7c00u) != 0x7c00u && (u & 0x7c000000u) != 0x7c000000u;
   }
 };
 
@@ -84,37 +70,6 @@ template <int N>
 __device__ __forceinline__ void cp_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
-// 2^x, to about 2 ulp (x <= 0 here; results below 2^-126 are 0)
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
-struct TreeArgs {
-  const void *q, *kc, *vc;
-  const int *table, *ctx, *cu;
-  const unsigned long long *mask;
-  void *out;
-  float *ws;
-  float scale_log2;  // scale * log2 e
-  int N, NQ, NKV, G, page, width, num_pages, S, max_q;
-};
-
-// Lengths of request b, held inside what the tensors have: queries within [0, N) and at most max_q, positions within
-// the table.
-struct Request {
-  int n0, T, ctx, len;
-  __device__ __forceinline__ Request(const TreeArgs &a, int b) {
-    const int c0 = __ldcg(a.cu + b), c1 = __ldcg(a.cu + b + 1);
-    n0 = min(max(c0, 0), a.N);
-    T = max(0, min(min(c1, a.N) - n0, a.max_q));
-    const long long room = (long long)a.width * a.page;
-    ctx = (int)min((long long)max(0, __ldcg(a.ctx + b)), room);
-    len = (int)min((long long)ctx + T, room);
-  }
-};
-
 // WM x WK warps: WM row groups of 16 MT rows, WK groups of 64 / WK keys of every tile (joined at the end).
 template <class T, int D, int WM, int WK, int MT, int STAGES>
 __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
@@ -125,6 +80,7 @@ __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
   constexpr int TILE = TA_KEYS * D * 2;  // bytes of a K (or V) tile
   extern __shared__ __align__(128) uint8_t ta_smem[];
   __shared__ int bad_pages;  // a page outside the pool was met
+  __shared__ int red;
   uint8_t *sk = ta_smem, *sv = ta_smem + STAGES * TILE, *sq = ta_smem + 2 * STAGES * TILE;
   pdl_trigger();
   pdl_wait();
@@ -133,8 +89,8 @@ __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
   const Request rq(a, b);
   const int rows = rq.T * a.G;
   if (r_base >= rows) return;
-  const int chunk = ((rq.len + a.S - 1) / a.S + TA_KEYS - 1) / TA_KEYS * TA_KEYS;
-  const int t0 = min((long long)split * chunk, (long long)rq.len), t1 = min(rq.len, t0 + chunk);
+  const int chunk = split_chunk(a, &red);
+  const int t0 = (int)min((long long)split * chunk, (long long)rq.len), t1 = t0 + min(rq.len - t0, chunk);
   const int tiles = (t1 - t0 + TA_KEYS - 1) / TA_KEYS;
   if (tid == 0) bad_pages = 0;
   __syncthreads();
@@ -197,6 +153,7 @@ __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
     }
   }
 
+  unsigned long long apart = 0;  // this warp's drafts that were taken out of the second product
   for (int it = 0; it < tiles; ++it) {
     cp_wait<STAGES - 2>();
     __syncthreads();  // the tile has landed for every warp, and the slot of tile it - 1 is free
@@ -286,56 +243,34 @@ __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
       }
     // ---------------------------------------------------------------- values
     // A draft that a row does not see has p = 0 there, but 0 times an infinity or a NaN is a NaN: drafts whose value
-    // row holds one are taken out of the product and added row by row where they are seen.
+    // row holds one are taken out of the product, and added at the end to the rows that see them.
     unsigned long long weird = 0;
     if (base + TA_KEYS > rq.ctx) {
 #pragma unroll
       for (int g = 0; g < (KW + 31) / 32; ++g) {
         bool w = false;
         const int r = k0 + g * 32 + lane;
-        if (g * 32 + lane < KW) {
+        if (g * 32 + lane < KW && base + r >= rq.ctx) {
 #pragma unroll 4
           for (int c = 0; c < CH; ++c) {
             const uint4 u = *reinterpret_cast<const uint4 *>(sv + slot * TILE + (r * CH + c) * 16);
-            w = w || !(Mma<T>::finite2(u.x) && Mma<T>::finite2(u.y) && Mma<T>::finite2(u.z) && Mma<T>::finite2(u.w));
+            w = w || !(Pair<T>::finite(u.x) && Pair<T>::finite(u.y) && Pair<T>::finite(u.z) && Pair<T>::finite(u.w));
           }
         }
         weird |= (unsigned long long)__ballot_sync(0xffffffffu, w) << (32 * g);
       }
-      for (unsigned long long left = weird; left; left &= left - 1) {
-        const int c = __ffsll(left) - 1, t = base + k0 + c, d = t - rq.ctx;
-        const int from = (lane & ~3) | ((c & 7) >> 1);
-        const uint32_t *vr = reinterpret_cast<const uint32_t *>(sv + slot * TILE) + (k0 + c) * CH * 4 + (lane & 3);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float p = 0.f;
-#pragma unroll
-            for (int j = 0; j < NB; ++j)
-              if (j == (c >> 3)) p = (c & 1) ? s[mt][j][2 * h + 1] : s[mt][j][2 * h];
-            p = __shfl_sync(0xffffffffu, p, from);
-            if (t < t1 && (d < 0 || ((see[mt][h] >> d) & 1))) {
-#pragma unroll
-              for (int j = 0; j < D / 8; ++j) {
-                const uint32_t u = vr[(j ^ ((k0 + c) & 7)) * 4];
-                const float2 v = Mma<T>::up2(u);
-                o[mt][j][2 * h] += p * v.x;
-                o[mt][j][2 * h + 1] += p * v.y;
-              }
-            }
-          }
-      }
+      const int d0 = base + k0 - rq.ctx;  // draft of the warp's first key (> -64)
+      apart |= d0 >= 0 ? weird << d0 : weird >> -d0;
     }
 #pragma unroll
     for (int kk = 0; kk < KW / 16; ++kk) {
       uint32_t pa[MT][4];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
-        pa[mt][0] = Mma<T>::pack(s[mt][2 * kk][0], s[mt][2 * kk][1]);
-        pa[mt][1] = Mma<T>::pack(s[mt][2 * kk][2], s[mt][2 * kk][3]);
-        pa[mt][2] = Mma<T>::pack(s[mt][2 * kk + 1][0], s[mt][2 * kk + 1][1]);
-        pa[mt][3] = Mma<T>::pack(s[mt][2 * kk + 1][2], s[mt][2 * kk + 1][3]);
+        pa[mt][0] = Pair<T>::pack(s[mt][2 * kk][0], s[mt][2 * kk][1]);
+        pa[mt][1] = Pair<T>::pack(s[mt][2 * kk][2], s[mt][2 * kk][3]);
+        pa[mt][2] = Pair<T>::pack(s[mt][2 * kk + 1][0], s[mt][2 * kk + 1][1]);
+        pa[mt][3] = Pair<T>::pack(s[mt][2 * kk + 1][2], s[mt][2 * kk + 1][3]);
       }
 #pragma unroll
       for (int jp = 0; jp < D / 16; ++jp) {
@@ -366,6 +301,37 @@ __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
       l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 1);
       l[mt][h] += __shfl_xor_sync(0xffffffffu, l[mt][h], 2);
     }
+
+  for (; apart; apart &= apart - 1) {  // rare: the score again from global memory, and p v added where it is seen
+    const int d = __ffsll(apart) - 1, t = rq.ctx + d;
+    const size_t at = (((size_t)page_of(t) * a.NKV + kvh) * a.page + t % a.page) * D;  // a page of the pool: it held
+    const T *kr = reinterpret_cast<const T *>(a.kc) + at, *vr = reinterpret_cast<const T *>(a.vc) + at;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int gr = r_base + wm * 16 * MT + mt * 16 + (lane >> 2) + 8 * h;
+        const T *qr = reinterpret_cast<const T *>(a.q) +
+                      ((size_t)(rq.n0 + (gr < rows ? gr / a.G : 0)) * a.NQ + kvh * a.G + (gr < rows ? gr % a.G : 0)) * D;
+        float dot = 0.f;
+        for (int j = lane & 3; j < D / 2; j += 4) {
+          const float2 x = Pair<T>::up(__ldcg(reinterpret_cast<const uint32_t *>(qr) + j));
+          const float2 y = Pair<T>::up(__ldcg(reinterpret_cast<const uint32_t *>(kr) + j));
+          dot += x.x * y.x + x.y * y.y;
+        }
+        dot += __shfl_xor_sync(0xffffffffu, dot, 1);
+        dot += __shfl_xor_sync(0xffffffffu, dot, 2);
+        if (gr < rows && ((see[mt][h] >> d) & 1)) {
+          const float p = ex2(fmaf(dot, a.scale_log2, m[mt][h] == -INFINITY ? 0.f : -m[mt][h]));
+#pragma unroll
+          for (int j = 0; j < D / 8; ++j) {
+            const float2 v = Pair<T>::up(__ldcg(reinterpret_cast<const uint32_t *>(vr) + 4 * j + (lane & 3)));
+            o[mt][j][2 * h] += p * v.x;
+            o[mt][j][2 * h + 1] += p * v.y;
+          }
+        }
+      }
+  }
 
   // ---------------------------------------------------------------- join the WK key groups of a row group
   if (WK > 1) {
@@ -422,7 +388,7 @@ __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
         const float inv = l[mt][h] == 0.f ? 0.f : 1.f / l[mt][h];
         uint32_t *dst = reinterpret_cast<uint32_t *>(reinterpret_cast<T *>(a.out) + row * D) + (lane & 3);
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) dst[4 * j] = Mma<T>::pack(o[mt][j][2 * h] * inv, o[mt][j][2 * h + 1] * inv);
+        for (int j = 0; j < D / 8; ++j) dst[4 * j] = Pair<T>::pack(o[mt][j][2 * h] * inv, o[mt][j][2 * h + 1] * inv);
       } else {
         float *w = a.ws + (row * a.S + split) * (D + 2);
         if ((lane & 3) == 0) *reinterpret_cast<float2 *>(w) = make_float2(m[mt][h], l[mt][h]);
@@ -457,6 +423,7 @@ __global__ void __launch_bounds__(32 * TC_WARPS) tree_combine_kernel(const TreeA
   for (int s = 0; s < a.S; ++s) {
     const float *p = w + (size_t)s * (D + 2);
     const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p));
+    if (ml.y == 0.f) continue;  // an empty split leaves its acc unwritten
     const float c = ex2(ml.x - ms);
     L += ml.y * c;
 #pragma unroll
@@ -469,7 +436,15 @@ __global__ void __launch_bounds__(32 * TC_WARPS) tree_combine_kernel(const TreeA
   const float inv = L == 0.f ? 0.f : 1.f / L;
   uint32_t *dst = reinterpret_cast<uint32_t *>(reinterpret_cast<T *>(a.out) + row * D + DPL * lane);
 #pragma unroll
-  for (int j = 0; j < DPL; j += 2) dst[j / 2] = Mma<T>::pack(acc[j] * inv, acc[j + 1] * inv);
+  for (int j = 0; j < DPL; j += 2) dst[j / 2] = Pair<T>::pack(acc[j] * inv, acc[j + 1] * inv);
+}
+
+template <class T, int D>
+cudaError_t launch_combine(const TreeArgs &a, bool pdl, cudaStream_t st) {
+  cudaLaunchAttribute attr;
+  const cudaLaunchConfig_t cfg =
+      pdl_config(dim3((a.max_q * a.NQ + TC_WARPS - 1) / TC_WARPS, a.B), dim3(32 * TC_WARPS), pdl, st, &attr);
+  return cudaLaunchKernelEx(&cfg, tree_combine_kernel<T, D>, a);
 }
 
 template <class T, int D, int WM, int WK, int MT, int STAGES>
@@ -488,9 +463,7 @@ cudaError_t launch_tile(const TreeArgs &a, int B, bool pdl, cudaStream_t st) {
                                       st, &attr);
   cfg.dynamicSmemBytes = SMEM;
   if (const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, a)) return e;
-  if (a.S == 1) return cudaSuccess;
-  cfg = pdl_config(dim3((a.max_q * a.NQ + TC_WARPS - 1) / TC_WARPS, B), dim3(32 * TC_WARPS), pdl, st, &attr);
-  return cudaLaunchKernelEx(&cfg, tree_combine_kernel<T, D>, a);
+  return a.S == 1 ? cudaSuccess : launch_combine<T, D>(a, pdl, st);
 }
 
 template <class T, int D>
@@ -519,7 +492,13 @@ cudaError_t launch_tree_attention(const void *q, const void *kc, const void *vc,
                                   int NKV, int D, int num_pages, int page, int width, int S, int max_q, float scale,
                                   bool half, bool pdl, cudaStream_t st) {
   const TreeArgs a{q, kc, vc, table, ctx, cu, reinterpret_cast<const unsigned long long *>(mask), out, ws,
-                   scale * 1.4426950408889634f, N, NQ, NKV, NQ / NKV, page, width, num_pages, S, max_q};
+                   scale * 1.4426950408889634f, N, B, NQ, NKV, NQ / NKV, page, width, num_pages, S, max_q};
+  if (page % 8 == 0) {
+    if (const cudaError_t e = launch_tree_tc(a, D, half, pdl, st)) return e;
+    if (S == 1) return cudaSuccess;
+    if (half) return D == 64 ? launch_combine<__half, 64>(a, pdl, st) : launch_combine<__half, 128>(a, pdl, st);
+    return D == 64 ? launch_combine<bf16, 64>(a, pdl, st) : launch_combine<bf16, 128>(a, pdl, st);
+  }
   if (half) return D == 64 ? launch_rows<__half, 64>(a, B, pdl, st) : launch_rows<__half, 128>(a, B, pdl, st);
   return D == 64 ? launch_rows<bf16, 64>(a, B, pdl, st) : launch_rows<bf16, 128>(a, B, pdl, st);
 }
