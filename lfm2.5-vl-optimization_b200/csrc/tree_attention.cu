@@ -390,16 +390,21 @@ __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
 #pragma unroll
         for (int j = 0; j < D / 8; ++j) dst[4 * j] = Pair<T>::pack(o[mt][j][2 * h] * inv, o[mt][j][2 * h + 1] * inv);
       } else {
-        float *w = a.ws + (row * a.S + split) * (D + 2);
-        if ((lane & 3) == 0) *reinterpret_cast<float2 *>(w) = make_float2(m[mt][h], l[mt][h]);
+        const float inv = l[mt][h] == 0.f ? 0.f : 1.f / l[mt][h];
+        float *w = ws_acc(a, D, split, row), *info = ws_row(a, D, row);
+        if ((lane & 3) == 0) {
+          info[1 + split] = l[mt][h] == 0.f ? -INFINITY : m[mt][h] + log2f(l[mt][h]);
+          if (split == 0) reinterpret_cast<int *>(info)[0] = a.S;
+        }
 #pragma unroll
         for (int j = 0; j < D / 8; ++j)
-          *reinterpret_cast<float2 *>(w + 2 + 8 * j + 2 * (lane & 3)) = make_float2(o[mt][j][2 * h], o[mt][j][2 * h + 1]);
+          *reinterpret_cast<float2 *>(w + 8 * j + 2 * (lane & 3)) =
+              make_float2(o[mt][j][2 * h] * inv, o[mt][j][2 * h + 1] * inv);
       }
     }
 }
 
-// One warp per (query, head): the S partials joined in split order.
+// One warp per (query, head): the parts joined in order. A row of one part has been written by its block.
 constexpr int TC_WARPS = 4;
 template <class T, int D>
 __global__ void __launch_bounds__(32 * TC_WARPS) tree_combine_kernel(const TreeArgs a) {
@@ -411,24 +416,24 @@ __global__ void __launch_bounds__(32 * TC_WARPS) tree_combine_kernel(const TreeA
   const Request rq(a, b);
   if (i >= rq.T) return;
   const size_t row = (size_t)(rq.n0 + i) * a.NQ + h;
-  const float *w = a.ws + row * a.S * (D + 2);
+  const float *info = ws_row(a, D, row);
+  const int parts = __ldcg(reinterpret_cast<const int *>(info));
+  if (parts <= 1) return;
   float M = -INFINITY;
-  for (int s = lane; s < a.S; s += 32) M = fmaxf(M, __ldcg(w + (size_t)s * (D + 2)));
+  for (int s = lane; s < parts; s += 32) M = fmaxf(M, __ldcg(info + 1 + s));
   M = warp_max(M);
   const float ms = M == -INFINITY ? 0.f : M;
   float L = 0.f, acc[DPL];
 #pragma unroll
   for (int j = 0; j < DPL; ++j) acc[j] = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < a.S; ++s) {
-    const float *p = w + (size_t)s * (D + 2);
-    const float2 ml = __ldcg(reinterpret_cast<const float2 *>(p));
-    if (ml.y == 0.f) continue;  // an empty split leaves its acc unwritten
-    const float c = ex2(ml.x - ms);
-    L += ml.y * c;
+  for (int s = 0; s < parts; ++s) {
+    const float c = ex2(__ldcg(info + 1 + s) - ms);
+    const float *p = ws_acc(a, D, s, row) + DPL * lane;
+    L += c;
 #pragma unroll
     for (int j = 0; j < DPL; j += 2) {
-      const float2 v = __ldcg(reinterpret_cast<const float2 *>(p + 2 + DPL * lane + j));
+      const float2 v = __ldcg(reinterpret_cast<const float2 *>(p + j));
       acc[j] += v.x * c;
       acc[j + 1] += v.y * c;
     }
@@ -479,12 +484,12 @@ cudaError_t launch_rows(const TreeArgs &a, int B, bool pdl, cudaStream_t st) {
 }  // namespace
 
 int tree_attention_splits(int B, int NQ, int NKV, int D, int max_q, long long max_len) {
-  // Enough splits to give every SM two blocks, but none shorter than four tiles.
-  const long long rows = (long long)max_q * (NQ / NKV), blocks = (long long)B * NKV * ((rows + 127) / 128);
-  const long long want = (2LL * device_sm_count() + blocks - 1) / blocks;
-  const long long most = (max_len + 4 * TA_KEYS - 1) / (4 * TA_KEYS);
+  // As many parts as equal stretches (two blocks an SM) cut a unit into, were all requests half as long as the longest;
+  // no more than a part a tile.
+  const long long per_tile = std::max(1, 128 / (NQ / NKV)), units = (long long)B * NKV * ((max_q + per_tile - 1) / per_tile);
+  const long long parts = 2 + (4LL * device_sm_count() + units - 1) / units, tiles = (max_len + TA_KEYS - 1) / TA_KEYS;
   (void)D;
-  return (int)std::max(1LL, std::min(std::min(want, most), 64LL));
+  return tiles <= 1 ? 1 : (int)std::min(std::min(parts, tiles + 1), 64LL);
 }
 
 cudaError_t launch_tree_attention(const void *q, const void *kc, const void *vc, const int *table, const int *ctx,

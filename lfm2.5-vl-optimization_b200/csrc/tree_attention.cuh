@@ -66,7 +66,7 @@ struct Request {
   }
 };
 
-// Keys per split, the same for every request (so that splits of long and short requests take the same time): the
+// Keys per split of the kernel for odd pages, the same for every request (so that splits of long and short requests take the same time): the
 // longest request cut into S, in whole tiles. For a whole block; `red` is one int of its shared memory.
 __device__ __forceinline__ int split_chunk(const TreeArgs &a, int *red) {
   if (threadIdx.x == 0) *red = 1;
@@ -77,6 +77,87 @@ __device__ __forceinline__ int split_chunk(const TreeArgs &a, int *red) {
   if ((threadIdx.x & 31) == 0) atomicMax(red, longest);
   __syncthreads();
   return ((*red + a.S - 1) / a.S + TA_KEYS - 1) / TA_KEYS * TA_KEYS;
+}
+
+// How the tensor-core kernel deals out work. A unit is one KV head and up to `rows` rows of one request; the tiles of all
+// units, in the order (request, KV head, row tile, position), are one line that is cut into equal stretches of `quota`
+// tiles, one a block: every block has the same work whatever the lengths, and a unit is split only where a stretch ends.
+// Every unit counts TA_UNIT_COST tiles more than it has, for its beginning and end in a block (about 3 us against 1 us a
+// tile: without it blocks with many short units ended last, 52 us where the mean was 38). No unit may fall into more
+// than S stretches: quota >= longest / (S - 1). With S = 1 whole units are dealt out.
+constexpr int TA_UNIT_COST = 3;
+struct TreePlan {
+  int rows;
+  long long quota;
+  int b;            // request of the block's first tile
+  long long base;   // tiles before that request
+  long long off;    // of the block's first tile within it
+  long long count;  // tiles of the block
+  static __device__ __forceinline__ int tiles(const Request &rq) { return (rq.len + TA_KEYS - 1) / TA_KEYS; }
+  // what a unit of n tiles takes of the line
+  static __device__ __forceinline__ int span(const TreeArgs &a, int n) { return a.S == 1 ? 1 : n + TA_UNIT_COST; }
+  __device__ __forceinline__ int units(const TreeArgs &a, const Request &rq) const {
+    return a.NKV * ((rq.T * a.G + rows - 1) / rows);
+  }
+  __device__ __forceinline__ long long weight(const TreeArgs &a, int i, int &n) const {
+    n = 0;
+    if (i >= a.B) return 0;
+    const Request rq(a, i);
+    if (rq.T == 0) return 0;
+    n = tiles(rq);
+    return (long long)units(a, rq) * span(a, n);
+  }
+  // For a whole warp: the stretch of block c of `blocks`.
+  __device__ __forceinline__ TreePlan(const TreeArgs &a, int rows_, int blocks, int c) : rows(rows_), b(a.B), base(0) {
+    const int lane = threadIdx.x & 31;
+    int longest = 1;
+    long long total = 0, first = 0;
+#pragma unroll 4
+    for (int i = lane; i < a.B; i += 32) {
+      int n;
+      const long long w = weight(a, i, n);
+      if (i == lane) first = w;
+      total += w;
+      longest = max(longest, n);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    longest = __reduce_max_sync(0xffffffffu, longest);
+    quota = (total + blocks - 1) / blocks;
+    if (a.S > 1) quota = max(quota, (long long)((longest + a.S - 2) / (a.S - 1)));
+    quota = max(quota, 1ll);
+    const long long x0 = quota * c;
+    count = max(0ll, min(quota, total - x0));
+    long long run = 0;
+    for (int b0 = 0; count > 0 && b0 < a.B; b0 += 32) {
+      int n;
+      const long long w = b0 == 0 ? first : weight(a, b0 + lane, n);
+      long long s = w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const long long s2 = __shfl_up_sync(0xffffffffu, s, o);
+        if (lane >= o) s += s2;
+      }
+      const uint32_t here = __ballot_sync(0xffffffffu, run + s - w <= x0 && x0 < run + s);
+      if (here) {  // one lane
+        const int at = __ffs(here) - 1;
+        b = b0 + at;
+        base = run + __shfl_sync(0xffffffffu, s - w, at);
+        break;
+      }
+      run += __shfl_sync(0xffffffffu, s, 31);
+    }
+    off = x0 - base;
+  }
+};
+
+// The workspace of a call with S > 1 splits: for every part of every row its accumulator divided by its sum, [S][N NQ]
+// [D], then per row 1 + S words: the number of parts, and each part's log2 of the sum of 2^score.
+__device__ __forceinline__ float *ws_acc(const TreeArgs &a, int D, int part, size_t row) {
+  return a.ws + ((size_t)part * a.N * a.NQ + row) * D;
+}
+__device__ __forceinline__ float *ws_row(const TreeArgs &a, int D, size_t row) {
+  return a.ws + (size_t)a.S * a.N * a.NQ * D + row * (1 + a.S);
 }
 
 // tree_attention_tc.cu

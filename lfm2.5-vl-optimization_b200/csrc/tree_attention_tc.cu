@@ -2,18 +2,16 @@
 // pages are multiples of 8 positions (tree_attention.cu has the mathematics, the form for other pages, and the join of
 // the splits).
 //
-// A block takes 128 rows (queries times heads of one KV head) of one request and one split of its positions. Warp 4
-// streams K and V tiles of 64 positions by TMA into 128-byte-swizzled stages (boxes of up to 64 rows that never cross
-// a page; one lane a box); warp 5 issues tcgen05.mma: S = Q K^T into one of two 64-column TMEM buffers, then
-// O += P V with P read back from TMEM (it lies over its S) and V as it is in the cache (an MN-major operand); warps 0-3
-// do the softmax, one thread a row, so that a row's maximum and sum need no exchange between lanes. While tile n is in
-// the softmax, S of tile n + 1 is computed and O of tile n - 1 accumulated. O stays in TMEM; it is rescaled only when a
-// row's maximum has grown by more than 2^8 since the last time (the probabilities then reach at most 2^8, exact as far
-// as floating point goes), which after the first tiles is rare.
-//
-// Per tile and row: 64 exponentials and about 4 times as many fp32 operations against 16 KB of K and V (head dim 64) a
-// block. 128 rows: bounded by the exponentials (16 a cycle and SM: 512 cycles a tile; 16 KB take 700 cycles of one SM's
-// share of the HBM rate), so two blocks an SM (96 KB of shared memory and 256 TMEM columns each) keep both busy.
+// A unit is a row tile (128 rows: queries times heads of one KV head) of one request, or two of them that share the K and
+// V tiles; the tiles of all units are one line that is cut into equal stretches, one a block (TreePlan). One warp works
+// out the block's stretches and streams them: the queries and K and V tiles of 64 positions by TMA into 128-byte-swizzled
+// stages (boxes of up to 64 rows that never cross a page; one lane a box). Per row tile one warp issues tcgen05.mma:
+// S = Q K^T into one of two 64-column TMEM buffers, then O += P V with P read from TMEM and V as it is in the cache (an
+// MN-major operand); four warps do the softmax, one thread a row, so that a row's maximum and sum need no exchange
+// between lanes. While tile n is in the softmax, S of tile n + 1 is ready, S of tile n + 2 follows as soon as tile n is
+// read, and O of tile n - 1 is accumulated. O stays in TMEM; it is rescaled only when a row's maximum has grown by more
+// than 2^8 since the last time (the probabilities then reach at most 2^8, as exact as below 1), rarely after the first
+// tiles.
 //
 // Every wait is bounded (about a second of SM clocks); a wait that gives up sets the device error word that
 // lfm2q_check_device reports, and the block ends without writing its rows.
@@ -35,10 +33,8 @@ __device__ int g_tree_err = 0;  // sticky: 1 = a pipeline wait gave up
 namespace {
 
 constexpr int TT_ROWS = 128;
-constexpr int TT_THREADS = 192;
 constexpr int TT_ATOM = TT_ROWS * 128;         // 64 dims of the query tile
 constexpr int TT_HALF = TA_KEYS * 128;         // 64 dims of a K (or V) tile
-constexpr int TT_TMEM = 256;                   // columns: S0 | S1 | O
 constexpr long long TT_WAIT_LIMIT = 1ll << 31;
 constexpr float TT_SLACK = 8.f;                // log2 of what a row's maximum may grow before O is rescaled
 
@@ -91,28 +87,32 @@ __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap *map
       : "memory");
 }
 // Operand in rows of 128 bytes, 128-byte swizzle, 8-row atoms 1024 bytes apart. lbo: MN-major operands wider than 64,
-// from one 64-wide block to the next (bytes).
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lbo) {
-  return (uint64_t)((saddr & 0x3FFFFu) >> 4) | (uint64_t)(lbo >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 |
-         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+// from one 64-wide block to the next (bytes). A descriptor is its low word (the address in 16-byte units and lbo), kept
+// in a register and stepped by additions, and one constant high word: the issuing thread's instructions are on the
+// pipeline's critical path (descriptors built anew for every MMA took 1000 of the 1900 cycles of a tile).
+__device__ __forceinline__ uint32_t sw128_lo(uint32_t saddr, uint32_t lbo) {
+  return ((saddr & 0x3FFFFu) >> 4) | (lbo >> 4) << 16;
 }
+constexpr uint32_t SW128_HI = (1024u >> 4) | 1u << 14 | 2u << 29;
 // kind::f16 instruction descriptor, fp32 accumulation, M = 128
 __host__ __device__ constexpr uint32_t idesc_f16(int n, bool bf, bool b_mn_major) {
   return (1u << 4) | (bf ? (1u << 7) | (1u << 10) : 0u) | (b_mn_major ? 1u << 16 : 0u) | ((uint32_t)(n >> 3) << 17) |
          ((uint32_t)(TT_ROWS >> 4) << 24);
 }
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_ss(uint32_t d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}" ::"r"(d),
+      "r"(a_lo), "r"(b_lo), "n"(SW128_HI), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint32_t b_lo, uint32_t idesc, uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
+      "mov.b64 db, {%2, %3};\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_lo), "n"(SW128_HI), "r"(idesc), "r"(accumulate)
       : "memory");
 }
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
@@ -149,312 +149,461 @@ __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
 }
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-template <int D>
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+
+// every lane of a warp waits
+__device__ __forceinline__ bool lanes_wait(uint32_t bar, uint32_t parity, volatile int *stop) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, stop));
+}
+
+template <int D, int PIPE>
 struct TcShape {
   static constexpr int HALVES = D / 64;
-  static constexpr int STAGES = D == 64 ? 5 : 2;
-  static constexpr int Q_BYTES = HALVES * TT_ATOM;
+  static constexpr int THREADS = 32 * (5 * PIPE + 1);  // per row tile four softmax warps and one that issues MMAs
+  // TMEM columns of a row tile: S0 | S1 | O (| P0 | P1 where there is room; else P lies over its S)
+  static constexpr bool OWN_P = D == 64;
+  static constexpr int O_COL = 2 * TA_KEYS, P_COL = O_COL + D;
+  static constexpr int STAGES = PIPE == 1 ? (D == 64 ? 5 : 2) : (D == 64 ? 8 : 4);
+  static constexpr int Q_BYTES = HALVES * TT_ATOM;   // per row tile
   static constexpr int KV_BYTES = HALVES * TT_HALF;  // a K (or V) tile
-  static constexpr int SMEM = Q_BYTES + 2 * STAGES * KV_BYTES + 1024;  // room to align the base to 1024
+  static constexpr int SMEM = PIPE * Q_BYTES + 2 * STAGES * KV_BYTES + 1024;  // room to align the base to 1024
 };
 
-template <class T, int D>
-__global__ void __launch_bounds__(TT_THREADS, 2)
-    tree_tc_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV, const TreeArgs a,
-                   int row_tiles, int box) {
-  using L = TcShape<D>;
+// A stretch of one unit's tiles. The loading warp works out the block's segments and hands each to the other warps in
+// shared memory together with its queries; tiles = 0 ends the block.
+struct Segment {
+  int b, kvh, tok0, n0;       // request, KV head, first query of the unit, the request's first row of q
+  int T, ctx, t0, tiles;      // queries and cached positions of the request; the stretch
+  int part, parts;            // which part of the unit this is, of how many
+};
+
+template <class T, int D, int PIPE>
+__global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
+    tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
+                   const __grid_constant__ CUtensorMap tmV, const TreeArgs a, int box, int tpt) {
+  using L = TcShape<D, PIPE>;
   constexpr int STAGES = L::STAGES, HALVES = L::HALVES;
   constexpr bool BF = std::is_same<T, bf16>::value;
+  constexpr int W_TMA = 4 * PIPE, W_MMA = W_TMA + 1;
+  constexpr int TMEM_COLS = 256 * PIPE;
   extern __shared__ uint8_t tt_smem[];
-  __shared__ __align__(8) uint64_t full_k[STAGES], full_v[STAGES], empty[STAGES], s_full[2], p_full[2], pv_done, o_full;
+  __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], q_full, q_empty, s_full[PIPE][2], p_full[PIPE][2],
+      pv_done[PIPE], o_full[PIPE], drained[PIPE];
   __shared__ unsigned long long live[STAGES];  // keys of the stage's tile that exist
-  __shared__ unsigned long long apart;         // drafts that were taken out of the second product
+  __shared__ unsigned long long apart[4];      // drafts that were taken out of the second product, by segment
+  __shared__ Segment segs[4];
   __shared__ uint32_t tmem_slot;
-  __shared__ int stop, red;
+  __shared__ int stop;
+  __shared__ int cleaned;  // tiles whose value rows the first warp has looked through
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tt_smem) + 1023) & ~uintptr_t(1023));
-  const uint32_t sq = smem_addr(smem), sk = sq + L::Q_BYTES, sv = sk + STAGES * L::KV_BYTES;
-  uint8_t *gv = smem + L::Q_BYTES + STAGES * L::KV_BYTES;  // the V stages, generic address
+  const uint32_t sq = smem_addr(smem), sk = sq + PIPE * L::Q_BYTES, sv = sk + STAGES * L::KV_BYTES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
-  pdl_wait();
-
-  const int rt = blockIdx.x % row_tiles, bk = blockIdx.x / row_tiles, kvh = bk % a.NKV, b = bk / a.NKV;
-  const int split = blockIdx.y, r_base = rt * TT_ROWS;
-  const Request rq(a, b);
-  const int rows = min(rq.T * a.G - r_base, TT_ROWS);
-  if (rows <= 0) return;
-  const int chunk = a.S == 1 ? (rq.len + TA_KEYS - 1) / TA_KEYS * TA_KEYS : split_chunk(a, &red);
-  const int t0 = (int)min((long long)split * chunk, (long long)rq.len), t1 = t0 + min(rq.len - t0, chunk);
-  const int tiles = (t1 - t0 + TA_KEYS - 1) / TA_KEYS;
-  const int row = threadIdx.x;  // warps 0-3: the thread's row of the tile
-  const int tok = (r_base + row) / a.G, head = kvh * a.G + (r_base + row) % a.G;
-  const size_t out_row = (size_t)(rq.n0 + tok) * a.NQ + head;
-  if (tiles == 0) {  // nothing to see here
-    if (row < rows) {
-      if (a.S == 1) {
-        uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + out_row * D);
-        for (int j = 0; j < D / 8; ++j) dst[j] = make_uint4(0, 0, 0, 0);
-      } else {
-        *reinterpret_cast<float2 *>(a.ws + (out_row * a.S + split) * (D + 2)) = make_float2(-INFINITY, 0.f);
-      }
-    }
-    return;
-  }
-  const int active = (rows + 31) / 32;  // softmax warps with rows
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
-      mbar_init(smem_addr(&full_k[i]), 1);
-      mbar_init(smem_addr(&full_v[i]), 1);
-      mbar_init(smem_addr(&empty[i]), 1);
+      mbar_init(smem_addr(&full[i]), 1);
+      mbar_init(smem_addr(&empty[i]), PIPE);
     }
-    for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_addr(&s_full[i]), 1);
-      mbar_init(smem_addr(&p_full[i]), active);
+    for (int p = 0; p < PIPE; ++p) {
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(smem_addr(&s_full[p][i]), 1);
+        mbar_init(smem_addr(&p_full[p][i]), 4);
+      }
+      mbar_init(smem_addr(&pv_done[p]), 1);
+      mbar_init(smem_addr(&o_full[p]), 1);
+      mbar_init(smem_addr(&drained[p]), 1);
     }
-    mbar_init(smem_addr(&pv_done), 1);
-    mbar_init(smem_addr(&o_full), 1);
-    stop = 0;
-    apart = 0;
+    mbar_init(smem_addr(&q_full), 1);
+    mbar_init(smem_addr(&q_empty), PIPE);
+    stop = cleaned = 0;
+    apart[0] = apart[1] = apart[2] = apart[3] = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == 5) {
+  if (warp == W_TMA && lane < 3)
+    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(lane == 0 ? &tmQ : lane == 1 ? &tmK : &tmV))
+                 : "memory");
+  if (warp == W_MMA) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&tmem_slot)),
-                 "r"(TT_TMEM)
+                 "r"(TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
-  // queries, in the swizzled layout of the first product's A operand; rows behind the last are zeros
-  for (int i = threadIdx.x; i < TT_ROWS * (D / 8); i += TT_THREADS) {
-    const int r = i / (D / 8), c = i % (D / 8), gr = r_base + r;
-    uint4 v = make_uint4(0, 0, 0, 0);
-    if (r < rows)
-      v = ld_cg16(reinterpret_cast<const T *>(a.q) +
-                  ((size_t)(rq.n0 + gr / a.G) * a.NQ + kvh * a.G + gr % a.G) * D + 8 * c);
-    *reinterpret_cast<uint4 *>(smem + (c >> 3) * TT_ATOM + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = v;
-  }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the generic writes, before the MMAs read them
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
-  const int *table = a.table + (size_t)b * a.width;
+  pdl_wait();
 
-  if (warp == 4) {
-    // ---------------------------------------------------------------- K and V tiles
+  if (warp == W_TMA) {
+    // ---------------------------------------------------------------- segments, queries, K and V tiles
+    const TreePlan plan(a, PIPE * tpt * a.G, gridDim.x, blockIdx.x);
     const int boxes = TA_KEYS / box;
-    int issued = 0;
-    for (int n = 0; n < tiles; ++n, ++issued) {
-      const int st = n % STAGES, base = t0 + n * TA_KEYS;
-      int pg[2], y[2];
-      uint32_t mine = 0;
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int i = lane + 32 * u, t = base + i * box;
-        pg[u] = -1;
-        if (i < boxes && t < t1) {
-          pg[u] = __ldcg(table + t / a.page);
-          y[u] = t % a.page;
+    long long left = plan.count, off = plan.off, base = plan.base;
+    int b = plan.b, st = 0, ph = 1;  // a fresh barrier passes a wait for the phase before its first
+    uint32_t issued = 0, seg = 0;
+    bool ok = true, more = true;
+    for (; ok && more; ++seg) {
+      more = false;
+      Segment g = {};
+      int t1 = 0;
+      while (left > 0 && b < a.B) {
+        const Request rq(a, b);
+        const int units = plan.units(a, rq), n = plan.tiles(rq), span = plan.span(a, n);
+        const long long w = (long long)units * span;
+        if (off >= w) {
+          base += w;
+          off = 0;
+          ++b;
+          continue;
         }
-        if (pg[u] < 0 || pg[u] >= a.num_pages) pg[u] = -1;
-        else ++mine;
+        // (the line fits 32 bits but for batches of some 10^9 tiles, whose divisions are slow)
+        const int unit = (int)(off < 0x7fffffff ? (int)off / span : off / span);
+        const int j0 = (int)(off - (long long)unit * span);
+        const int step = (int)min((long long)(span - j0), left), per_head = units / a.NKV;
+        off += step;
+        left -= step;
+        const int take = a.S == 1 ? n : min(n - j0, step);
+        if (take <= 0) continue;  // the end of a unit's span holds no tiles
+        long long part = 0, last = 0;
+        if (a.S > 1) {
+          const long long first = base + off - step - j0, q = plan.quota;  // the unit's first tile in the line
+          if (first + n < 0x7fffffff && q < 0x7fffffff) {
+            const int f = (int)first / (int)q;
+            part = ((int)first + j0) / (int)q - f;
+            last = ((int)first + n - 1) / (int)q - f;
+          } else {
+            part = (first + j0) / q - first / q;
+            last = (first + n - 1) / q - first / q;
+          }
+        }
+        g = {b, unit / per_head, unit % per_head * PIPE * tpt, rq.n0, rq.T, rq.ctx, j0 * TA_KEYS, take, (int)part,
+             (int)last + 1};
+        t1 = min(rq.len, (j0 + take) * TA_KEYS);
+        more = true;
+        break;
       }
-      const uint32_t loads = __reduce_add_sync(0xffffffffu, mine);
-      unsigned long long keys = 0;  // of this lane's boxes
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (pg[u] >= 0) {
-          const int i = lane + 32 * u, n_live = min(box, t1 - (base + i * box));
-          keys |= (n_live >= 64 ? ~0ull : (1ull << n_live) - 1) << (i * box);
-        }
-      const uint32_t klo = __reduce_or_sync(0xffffffffu, (uint32_t)keys),
-                     khi = __reduce_or_sync(0xffffffffu, (uint32_t)(keys >> 32));
-      if (n >= STAGES && !warp_wait(smem_addr(&empty[st]), (uint32_t)((n / STAGES - 1) & 1), &stop)) break;
-      const uint32_t fk = smem_addr(&full_k[st]), fv = smem_addr(&full_v[st]);
+      // the queries' place is free when the last scores of the segment before are done
+      ok = warp_wait(smem_addr(&q_empty), (seg & 1) ^ 1, &stop);
+      if (!ok) break;
       if (lane == 0) {
-        live[st] = (unsigned long long)khi << 32 | klo;
-        mbar_expect_tx(fk, loads * box * 128 * HALVES);
-        mbar_expect_tx(fv, loads * box * 128 * HALVES);
+        segs[seg & 3] = g;
+        const int tiles_q = more ? min(PIPE, (g.T - g.tok0 + tpt - 1) / tpt) : 0;
+        mbar_expect_tx(smem_addr(&q_full), tiles_q * HALVES * tpt * a.G * 128);
+        for (int p = 0; p < tiles_q; ++p)
+          for (int h = 0; h < HALVES; ++h)
+            tma_load_3d(sq + p * L::Q_BYTES + h * TT_ATOM, &tmQ, smem_addr(&q_full), 64 * h, g.kvh * a.G,
+                        g.n0 + g.tok0 + p * tpt);
       }
-      __syncwarp();
+      const int *table = a.table + (size_t)g.b * a.width;
+      for (int n = 0; n < g.tiles; ++n, ++issued) {
+        const int tile_at = g.t0 + n * TA_KEYS;
+        int pg[2], y[2] = {0, 0};
+        uint32_t mine = 0;
+        unsigned long long keys = 0;  // of this lane's boxes
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (pg[u] >= 0)
+        for (int u = 0; u < 2; ++u) {
+          const int i = lane + 32 * u, t = tile_at + i * box;
+          pg[u] = -1;
+          if (i < boxes && t < t1) {
+            pg[u] = __ldcg(table + t / a.page);
+            y[u] = t % a.page;
+          }
+          if (pg[u] < 0 || pg[u] >= a.num_pages) {
+            pg[u] = -1;
+          } else {
+            ++mine;
+            const int n_live = min(box, t1 - t);
+            keys |= (n_live >= 64 ? ~0ull : (1ull << n_live) - 1) << (i * box);
+          }
+        }
+        const uint32_t loads = __reduce_add_sync(0xffffffffu, mine);
+        const uint32_t klo = __reduce_or_sync(0xffffffffu, (uint32_t)keys),
+                       khi = __reduce_or_sync(0xffffffffu, (uint32_t)(keys >> 32));
+        ok = warp_wait(smem_addr(&empty[st]), (uint32_t)ph, &stop);
+        if (!ok) break;
+        const uint32_t bar = smem_addr(&full[st]);
+        if (lane == 0) {
+          live[st] = (unsigned long long)khi << 32 | klo;
+          mbar_expect_tx(bar, 2 * loads * box * 128 * HALVES);
+        }
+        __syncwarp();
 #pragma unroll
-          for (int h = 0; h < HALVES; ++h)
-            tma_load_3d(sk + st * L::KV_BYTES + h * TT_HALF + (lane + 32 * u) * box * 128, &tmK, fk, 64 * h, y[u],
-                        pg[u] * a.NKV + kvh);
+        for (int u = 0; u < 2; ++u)
+          if (pg[u] >= 0)
 #pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (pg[u] >= 0)
+            for (int h = 0; h < HALVES; ++h)
+              tma_load_3d(sk + st * L::KV_BYTES + h * TT_HALF + (lane + 32 * u) * box * 128, &tmK, bar, 64 * h, y[u],
+                          pg[u] * a.NKV + g.kvh);
 #pragma unroll
-          for (int h = 0; h < HALVES; ++h)
-            tma_load_3d(sv + st * L::KV_BYTES + h * TT_HALF + (lane + 32 * u) * box * 128, &tmV, fv, 64 * h, y[u],
-                        pg[u] * a.NKV + kvh);
+        for (int u = 0; u < 2; ++u)
+          if (pg[u] >= 0)
+#pragma unroll
+            for (int h = 0; h < HALVES; ++h)
+              tma_load_3d(sv + st * L::KV_BYTES + h * TT_HALF + (lane + 32 * u) * box * 128, &tmV, bar, 64 * h, y[u],
+                          pg[u] * a.NKV + g.kvh);
+        if (++st == STAGES) {
+          st = 0;
+          ph ^= 1;
+        }
+      }
     }
-    if (issued < tiles && lane == 0) {  // gave up: no copy may land after the block has left
+    if (!ok && lane == 0) {  // gave up: no copy may land after the block has left
       int late = 0;
-      for (int n = max(0, issued - STAGES); n < issued; ++n) {
-        mbar_wait(smem_addr(&full_k[n % STAGES]), (uint32_t)((n / STAGES) & 1), &late);
-        mbar_wait(smem_addr(&full_v[n % STAGES]), (uint32_t)((n / STAGES) & 1), &late);
+      for (uint32_t n = issued > STAGES ? issued - STAGES : 0; n < issued; ++n) {
+        mbar_wait(smem_addr(&full[n % STAGES]), (n / STAGES) & 1, &late);
       }
+      if (seg > 0) mbar_wait(smem_addr(&q_full), (seg - 1) & 1, &late);
     }
-  } else if (warp == 5) {
-    // ---------------------------------------------------------------- MMAs
+  } else if (warp >= W_MMA) {
+    // ---------------------------------------------------------------- MMAs of row tile p
+    // One thread issues them, and what it does a tile (waits of 100 cycles, MMAs of 60, commits of 80) bounds the tile
+    // when it is much: so a warp of its own for every row tile, one barrier for K and V, and no wait that the order of
+    // the MMAs makes needless.
     if (lane == 0) {
       constexpr uint32_t ID_S = idesc_f16(TA_KEYS, BF, false), ID_O = idesc_f16(D, BF, true);
-      auto scores = [&](int n) {
-        const int st = n % STAGES;
-        // P of tile n - 2 lies in this buffer until its product is done
-        if (n >= 2 && !mbar_wait(smem_addr(&pv_done), (uint32_t)(n & 1), &stop)) return false;
-        if (!mbar_wait(smem_addr(&full_k[st]), (uint32_t)((n / STAGES) & 1), &stop)) return false;
+      const int p = warp - W_MMA;
+      const uint32_t q_lo = sw128_lo(sq + p * L::Q_BYTES, 16), k_lo = sw128_lo(sk, 16), v_lo = sw128_lo(sv, TT_HALF);
+      const uint32_t t_s = tmem + 256 * p, t_o = t_s + L::O_COL, t_p = L::OWN_P ? t_s + L::P_COL : t_s;
+      constexpr uint32_t P_STEP = L::OWN_P ? TA_KEYS / 2 : TA_KEYS;
+      int kst = 0, kph = 0, st = 0;  // stage and phase of the next scores' tile, stage of the next product's
+      uint32_t cnt = 0, seg = 0;     // tiles and segments so far
+      bool ok = true;
+      auto scores = [&](uint32_t i) {
+        ok = mbar_wait(smem_addr(&full[kst]), (uint32_t)kph, &stop);
+        if (!ok) return;
         tc_fence_after();
+        const uint32_t kt = k_lo + kst * (L::KV_BYTES / 16);
 #pragma unroll
         for (int k = 0; k < D / 16; ++k)
-          umma_ss(tmem + (n & 1) * TA_KEYS, sw128_desc(sq + (k >> 2) * TT_ATOM, 16) + 2 * (k & 3),
-                  sw128_desc(sk + st * L::KV_BYTES + (k >> 2) * TT_HALF, 16) + 2 * (k & 3), ID_S, k != 0);
-        umma_commit(smem_addr(&s_full[n & 1]));
-        return true;
-      };
-      bool ok = scores(0);
-      for (int n = 0; n < tiles && ok; ++n) {
-        const int st = n % STAGES;
-        ok = (n + 1 >= tiles || scores(n + 1)) &&
-             mbar_wait(smem_addr(&p_full[n & 1]), (uint32_t)((n >> 1) & 1), &stop) &&
-             mbar_wait(smem_addr(&full_v[st]), (uint32_t)((n / STAGES) & 1), &stop);
-        if (!ok) break;
-        tc_fence_after();
-#pragma unroll
-        for (int k = 0; k < TA_KEYS / 16; ++k)
-          umma_ts(tmem + 2 * TA_KEYS, tmem + (n & 1) * TA_KEYS + 8 * k,
-                  sw128_desc(sv + st * L::KV_BYTES + k * 2048, TT_HALF), ID_O, (n | k) != 0);
-        umma_commit(smem_addr(&empty[st]));
-        umma_commit(smem_addr(&pv_done));
-      }
-      umma_commit(smem_addr(&o_full));
-      int late = 0;
-      if (!ok) mbar_wait(smem_addr(&o_full), 0, &late);  // gave up: the MMAs in flight finish first
-    }
-  } else if (warp < active) {
-    // ---------------------------------------------------------------- softmax, one thread a row
-    const uint32_t lane_at = (uint32_t)(warp * 32) << 16;
-    unsigned long long see = 0;
-    if (row < rows) see = a.mask ? __ldcg(a.mask + rq.n0 + tok) : (tok >= 63 ? ~0ull : (2ull << tok) - 1);
-    float m = -INFINITY, l = 0.f;
-    bool ok = true;
-    for (int n = 0; n < tiles; ++n) {
-      const int st = n % STAGES, base = t0 + n * TA_KEYS;
-      const uint32_t sbuf = tmem + lane_at + (n & 1) * TA_KEYS;
-      ok = warp_wait(smem_addr(&s_full[n & 1]), (uint32_t)((n >> 1) & 1), &stop);
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t s0[32], s1[32];
-      tmem_ld32(sbuf, s0);
-      tmem_ld32(sbuf + 32, s1);
-      // keys of the tile that this row sees
-      unsigned long long vis = *(volatile unsigned long long *)&live[st];
-      const unsigned long long exists = vis;
-      const int d0 = base - rq.ctx;  // draft of the tile's first key
-      if (d0 > -TA_KEYS) vis &= d0 >= 0 ? (d0 < 64 ? see >> d0 : 0ull) : (1ull << -d0) - 1 | see << -d0;
-      tmem_ld_wait(s0);
-      tmem_ld_wait(s1);
-      if (__any_sync(0xffffffffu, vis != ~0ull)) {
-        const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          if (!((v0 >> j) & 1)) s0[j] = 0xff800000u;
-          if (!((v1 >> j) & 1)) s1[j] = 0xff800000u;
+          umma_ss(t_s + i * TA_KEYS, q_lo + (k >> 2) * (TT_ATOM / 16) + 2 * (k & 3),
+                  kt + (k >> 2) * (TT_HALF / 16) + 2 * (k & 3), ID_S, k != 0);
+        umma_commit(smem_addr(&s_full[p][i]));
+        if (++kst == STAGES) {
+          kst = 0;
+          kph ^= 1;
         }
-      }
-      float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-      for (int j = 0; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], fmaxf(__uint_as_float(s0[j]), __uint_as_float(s1[j])));
-      const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
-      const bool grow = top > m + TT_SLACK || (m == -INFINITY && top > -INFINITY);
-      if (__any_sync(0xffffffffu, grow)) {
-        const float corr = grow ? ex2(m - top) : 1.f;  // 0 while the row has seen nothing
-        if (grow) m = top;
-        l *= corr;
-        if (n > 0) {
-          ok = warp_wait(smem_addr(&pv_done), (uint32_t)((n - 1) & 1), &stop);
+      };
+      for (;; ++seg) {
+        ok = mbar_wait(smem_addr(&q_full), seg & 1, &stop);
+        if (!ok) break;
+        const int tiles = *(volatile int *)&segs[seg & 3].tiles;
+        if (tiles == 0) break;
+        // Scores run two tiles ahead of the softmax's end, so that it always finds the next tile ready.
+        scores(cnt & 1);
+        if (ok && tiles > 1) scores((cnt + 1) & 1);
+        for (int n = 0; n < tiles && ok; ++n, ++cnt) {
+          const uint32_t i = cnt & 1;
+          ok = mbar_wait(smem_addr(&p_full[p][i]), (cnt >> 1) & 1, &stop);
           if (!ok) break;
           tc_fence_after();
+          const uint32_t vt = v_lo + st * (L::KV_BYTES / 16), pt = t_p + i * P_STEP;
 #pragma unroll
-          for (int c = 0; c < D / 32; ++c) {
-            uint32_t o[32];
-            tmem_ld32(tmem + lane_at + 2 * TA_KEYS + 32 * c, o);
-            tmem_ld_wait(o);
-#pragma unroll
-            for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
-            tmem_st32(tmem + lane_at + 2 * TA_KEYS + 32 * c, o);
+          for (int k = 0; k < TA_KEYS / 16; ++k) umma_ts(t_o, pt + 8 * k, vt + k * (2048 / 16), ID_O, (n | k) != 0);
+          umma_commit(smem_addr(&empty[st]));
+          if (n == tiles - 1) umma_commit(smem_addr(&o_full[p]));
+          if (!L::OWN_P || n == tiles - 2) umma_commit(smem_addr(&pv_done[p]));
+          if (n + 2 < tiles) {
+            // S of tile n + 2 goes where tile n's was: read by the softmax (p_full), and where P lies over it multiplied
+            if (!L::OWN_P) ok = mbar_wait(smem_addr(&pv_done[p]), i, &stop);
+            if (ok) scores(i);
+          } else if (!L::OWN_P) {
+            ok = mbar_wait(smem_addr(&pv_done[p]), i, &stop);
           }
+          // the queries have been read; not before the softmax has taken this segment up (its barrier then is at most
+          // one phase ahead of any waiter)
+          if (ok && n == max(tiles - 3, 0)) umma_commit(smem_addr(&q_empty));
+          if (++st == STAGES) st = 0;
         }
-      }
-      const float ms = m == -INFINITY ? 0.f : m;
-      uint32_t p[32];
-      float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        const float e0 = ex2(fmaf(__uint_as_float(s0[2 * j]), a.scale_log2, -ms));
-        const float e1 = ex2(fmaf(__uint_as_float(s0[2 * j + 1]), a.scale_log2, -ms));
-        const float f0 = ex2(fmaf(__uint_as_float(s1[2 * j]), a.scale_log2, -ms));
-        const float f1 = ex2(fmaf(__uint_as_float(s1[2 * j + 1]), a.scale_log2, -ms));
-        p[j] = Pair<T>::pack(e0, e1);
-        p[16 + j] = Pair<T>::pack(f0, f1);
-        sum[0] += e0;
-        sum[1] += e1;
-        sum[2] += f0;
-        sum[3] += f1;
-      }
-      l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-      tmem_st32(sbuf, p);
-      // A key that a row does not see has p = 0, but 0 times an infinity or a NaN is a NaN: value rows that hold one
-      // are zeroed in shared memory (stale ones of keys that do not exist, too), and drafts among them are added at
-      // the end to the rows that see them.
-      if (warp == 0 && (d0 > -TA_KEYS || exists != ~0ull)) {
-        ok = warp_wait(smem_addr(&full_v[st]), (uint32_t)((n / STAGES) & 1), &stop);
         if (!ok) break;
-#pragma unroll
-        for (int g = 0; g < 2; ++g) {
-          const int r = g * 32 + lane;
-          uint4 *vr = reinterpret_cast<uint4 *>(gv + st * L::KV_BYTES + r * 128);
-          bool bad = false;
-          if (base + r >= rq.ctx || !((exists >> r) & 1)) {
-            for (int h = 0; h < HALVES; ++h)
-              for (int c = 0; c < 8; ++c) {
-                const uint4 u = vr[h * (TT_HALF / 16) + c];
-                bad = bad || !(Pair<T>::finite(u.x) && Pair<T>::finite(u.y) && Pair<T>::finite(u.z) && Pair<T>::finite(u.w));
-              }
-            if (bad)
-              for (int h = 0; h < HALVES; ++h)
-                for (int c = 0; c < 8; ++c) vr[h * (TT_HALF / 16) + c] = make_uint4(0, 0, 0, 0);
-          }
-          if (bad && ((exists >> r) & 1)) atomicOr(&apart, 1ull << (base + r - rq.ctx));
-        }
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       }
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_addr(&p_full[n & 1]));
+      if (!ok) {  // gave up: the MMAs in flight finish first
+        int late = 0;
+        umma_commit(smem_addr(&drained[p]));
+        mbar_wait(smem_addr(&drained[p]), 0, &late);
+      }
     }
-    // ---------------------------------------------------------------- out, or this split's partial
-    ok = ok && warp_wait(smem_addr(&o_full), 0, &stop) && *(volatile int *)&stop == 0;
-    ok = __all_sync(0xffffffffu, ok);
-    if (ok) {
+  } else {
+    // ---------------------------------------------------------------- softmax, one thread a row
+    const int pipe = warp >> 2, quarter = warp & 3, row = threadIdx.x & (TT_ROWS - 1);
+    const uint32_t tbase = tmem + 256 * pipe + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t t_o = tbase + L::O_COL;
+    uint32_t cnt = 0, seg = 0, pairs = 0;  // tiles, segments, segments of two tiles or more
+    int st = 0, ph = 0, edges = 0;
+    bool ok = true;
+    for (;; ++seg) {
+      ok = lanes_wait(smem_addr(&q_full), seg & 1, &stop);
+      if (!ok) break;
+      const volatile Segment *g = &segs[seg & 3];
+      const int tiles = g->tiles, ctx = g->ctx, t0 = g->t0;
+      if (tiles == 0) break;
+      const int tok0 = g->tok0 + pipe * tpt, toks = min(g->T - tok0, tpt);  // this row tile's queries (none: <= 0)
+      const bool active = quarter * 32 < toks * a.G, has = row < toks * a.G;
+      unsigned long long see = 0;
+      if (has) {
+        const int tok = tok0 + row / a.G;
+        see = a.mask ? __ldcg(a.mask + g->n0 + tok) : (tok >= 63 ? ~0ull : (2ull << tok) - 1);
+      }
+      float m = -INFINITY, l = 0.f;
+      for (int n = 0; n < tiles; ++n, ++cnt) {
+        const uint32_t sbuf = tbase + (cnt & 1) * TA_KEYS;
+        const uint32_t pbuf = L::OWN_P ? tbase + L::P_COL + (cnt & 1) * (TA_KEYS / 2) : sbuf;
+        const uint32_t pbar = smem_addr(&p_full[pipe][cnt & 1]);
+        ok = lanes_wait(smem_addr(&s_full[pipe][cnt & 1]), (cnt >> 1) & 1, &stop);
+        if (!ok) break;
+        const unsigned long long exists = *(volatile unsigned long long *)&live[st];
+        const int d0 = t0 + n * TA_KEYS - ctx;  // draft of the tile's first key
+        const bool edge = d0 > -TA_KEYS || exists != ~0ull;
+        edges += edge;
+        if (!active) {
+          if (lane == 0) mbar_arrive(pbar);  // keeps step: a row tile's barriers count all four warps
+        } else {
+          tc_fence_after();
+          uint32_t s0[32], s1[32];
+          tmem_ld32(sbuf, s0);
+          tmem_ld32(sbuf + 32, s1);
+          unsigned long long vis = exists;  // keys of the tile that this row sees
+          if (d0 > -TA_KEYS) vis &= d0 >= 0 ? (d0 < 64 ? see >> d0 : 0ull) : (1ull << -d0) - 1 | see << -d0;
+          tmem_ld_wait(s0);
+          tmem_ld_wait(s1);
+          if (__any_sync(0xffffffffu, vis != ~0ull)) {
+            const uint32_t v0 = (uint32_t)vis, v1 = (uint32_t)(vis >> 32);
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (!((v0 >> j) & 1)) s0[j] = 0xff800000u;
+              if (!((v1 >> j) & 1)) s1[j] = 0xff800000u;
+            }
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) mx[j & 3] = max3(mx[j & 3], __uint_as_float(s0[j]), __uint_as_float(s1[j]));
+          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          const bool grow = top > m + TT_SLACK || (m == -INFINITY && top > -INFINITY);
+          if (__any_sync(0xffffffffu, grow)) {
+            const float corr = grow ? ex2(m - top) : 1.f;  // 0 while the row has seen nothing
+            if (grow) m = top;
+            l *= corr;
+            if (n > 0) {
+              // the product of tile n - 1: done when S of tile n + 1 is, which was issued after it
+              ok = !L::OWN_P ? lanes_wait(smem_addr(&pv_done[pipe]), (cnt - 1) & 1, &stop)
+                   : n + 1 < tiles
+                       ? lanes_wait(smem_addr(&s_full[pipe][(cnt + 1) & 1]), ((cnt + 1) >> 1) & 1, &stop)
+                       : lanes_wait(smem_addr(&pv_done[pipe]), pairs & 1, &stop);
+              if (!ok) break;
+              tc_fence_after();
+#pragma unroll
+              for (int c = 0; c < D / 32; ++c) {
+                uint32_t o[32];
+                tmem_ld32(t_o + 32 * c, o);
+                tmem_ld_wait(o);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * corr);
+                tmem_st32(t_o + 32 * c, o);
+              }
+            }
+          }
+          const float ms = m == -INFINITY ? 0.f : m;
+          const float2 c2 = make_float2(a.scale_log2, a.scale_log2), m2 = make_float2(-ms, -ms);
+          uint32_t p[32];
+          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const float2 x = ffma2(make_float2(__uint_as_float(s0[2 * j]), __uint_as_float(s0[2 * j + 1])), c2, m2);
+            const float2 y = ffma2(make_float2(__uint_as_float(s1[2 * j]), __uint_as_float(s1[2 * j + 1])), c2, m2);
+            const float2 e = make_float2(ex2(x.x), ex2(x.y)), f = make_float2(ex2(y.x), ex2(y.y));
+            p[j] = Pair<T>::pack(e.x, e.y);
+            p[16 + j] = Pair<T>::pack(f.x, f.y);
+            sum0 = fadd2(sum0, e);
+            sum1 = fadd2(sum1, f);
+          }
+          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+          tmem_st32(pbuf, p);
+          // A key that a row does not see has p = 0, but 0 times an infinity or a NaN is a NaN: value rows that hold
+          // one are zeroed in shared memory (stale ones of keys that do not exist, too), and drafts among them are
+          // added at the end to the rows that see them. The first warp does it, and the other row tile's first warp
+          // waits for it, before they let the product go ahead.
+          if (edge && warp == 0) {
+            ok = lanes_wait(smem_addr(&full[st]), (uint32_t)ph, &stop);  // it has landed: S came of it
+            if (!ok) break;
+#pragma unroll
+            for (int h2 = 0; h2 < 2; ++h2) {
+              const int r = h2 * 32 + lane;
+              const bool there = (exists >> r) & 1;
+              const bool look = d0 + r >= 0 || !there;
+              if (!__any_sync(0xffffffffu, look)) continue;
+              uint4 *vr = reinterpret_cast<uint4 *>(smem + PIPE * L::Q_BYTES + STAGES * L::KV_BYTES + st * L::KV_BYTES +
+                                                    r * 128);
+              bool bad = false;
+              for (int h = 0; h < HALVES; ++h)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) {  // every lane at another 16 bytes of its row: no bank twice
+                  const uint4 u = vr[h * (TT_HALF / 16) + ((c + lane) & 7)];
+                  bad = bad ||
+                        !(Pair<T>::finite(u.x) && Pair<T>::finite(u.y) && Pair<T>::finite(u.z) && Pair<T>::finite(u.w));
+                }
+              if (bad && look) {
+                for (int h = 0; h < HALVES; ++h)
+                  for (int c = 0; c < 8; ++c) vr[h * (TT_HALF / 16) + c] = make_uint4(0, 0, 0, 0);
+                if (there) atomicOr(&apart[seg & 3], 1ull << (d0 + r));
+              }
+            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            __syncwarp();
+            if (PIPE > 1 && lane == 0) {
+              __threadfence_block();
+              *(volatile int *)&cleaned = edges;
+            }
+          } else if (PIPE > 1 && edge && warp == 4) {
+            const long long since = clock64();
+            while (ok && *(volatile int *)&cleaned < edges)
+              ok = *(volatile int *)&stop == 0 && clock64() - since < TT_WAIT_LIMIT;
+            ok = __all_sync(0xffffffffu, ok);
+            __threadfence_block();
+            if (!ok) {
+              stop = 1;
+              atomicCAS(&g_tree_err, 0, 1);
+              break;
+            }
+          }
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(pbar);
+        }
+        if (++st == STAGES) {
+          st = 0;
+          ph ^= 1;
+        }
+      }
+      pairs += tiles > 1;
+      // ---------------------------------------------------------------- out, or this split's partial
+      ok = ok && lanes_wait(smem_addr(&o_full[pipe]), seg & 1, &stop) && *(volatile int *)&stop == 0;
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+      // The word of two segments on: every row tile has left the segment two back, whose word that was (this one's
+      // last product came after all of the last one's, whose P came after that).
+      if (warp == 0 && lane == 0) apart[(seg + 2) & 3] = 0;
+      if (!active) continue;
       tc_fence_after();
+      const int parts = g->parts;
+      const size_t out_row = (size_t)(g->n0 + tok0 + row / a.G) * a.NQ + g->kvh * a.G + row % a.G;
       const float inv = l == 0.f ? 0.f : 1.f / l;
-      const unsigned long long extra = *(volatile unsigned long long *)&apart & see;
-      float *part = a.ws + (out_row * a.S + split) * (D + 2);
+      const unsigned long long extra = *(volatile unsigned long long *)&apart[seg & 3] & see;
+      float *part = ws_acc(a, D, g->part, out_row);
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
         uint32_t o[32];
-        tmem_ld32(tmem + lane_at + 2 * TA_KEYS + 32 * c, o);
+        tmem_ld32(t_o + 32 * c, o);
         tmem_ld_wait(o);
-        if (extra && row < rows) {  // rare: the score again from global memory, and p v added
+        if (extra && has) {  // rare: the score again from global memory, and p v added
           const uint32_t *qr = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(a.q) + out_row * D);
-          for (unsigned long long left = extra; left; left &= left - 1) {
-            const int t = rq.ctx + __ffsll(left) - 1;
-            const size_t at = (((size_t)__ldcg(table + t / a.page) * a.NKV + kvh) * a.page + t % a.page) * D;
+          for (unsigned long long rest = extra; rest; rest &= rest - 1) {
+            const int t = ctx + __ffsll(rest) - 1;
+            const size_t at =
+                (((size_t)__ldcg(a.table + (size_t)g->b * a.width + t / a.page) * a.NKV + g->kvh) * a.page + t % a.page) * D;
             const uint32_t *kr = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(a.kc) + at);
             const uint32_t *vr = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(a.vc) + at) + 16 * c;
             float dot = 0.f;
@@ -471,34 +620,40 @@ __global__ void __launch_bounds__(TT_THREADS, 2)
             }
           }
         }
-        if (row < rows) {
-          if (a.S == 1) {
+#pragma unroll
+        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * inv);
+        if (has) {
+          if (parts == 1) {
             uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + out_row * D + 32 * c);
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
               uint32_t w[4];
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                w[e] = Pair<T>::pack(__uint_as_float(o[8 * j + 2 * e]) * inv, __uint_as_float(o[8 * j + 2 * e + 1]) * inv);
+                w[e] = Pair<T>::pack(__uint_as_float(o[8 * j + 2 * e]), __uint_as_float(o[8 * j + 2 * e + 1]));
               dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
             }
           } else {
+            uint4 *dst = reinterpret_cast<uint4 *>(part + 32 * c);
 #pragma unroll
-            for (int j = 0; j < 16; ++j)
-              *reinterpret_cast<float2 *>(part + 2 + 32 * c + 2 * j) =
-                  make_float2(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
+            for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
           }
         }
       }
-      if (a.S > 1 && row < rows) *reinterpret_cast<float2 *>(part) = make_float2(m, l);
+      if (a.S > 1 && has) {
+        float *info = ws_row(a, D, out_row);
+        if (parts > 1) info[1 + g->part] = l == 0.f ? -INFINITY : m + log2f(l);
+        if (g->part == 0) reinterpret_cast<int *>(info)[0] = parts;
+      }
+      tc_fence_before();  // O has been read, before the next segment's first product (ordered by its P)
     }
   }
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
+  if (warp == W_MMA) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TT_TMEM) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
   }
 }
 
@@ -515,42 +670,50 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// cache [heads, page, D] (heads = num_pages * NKV), box = 64 dims x box rows of one page, 128-byte swizzle
-bool make_map(CUtensorMap *map, const void *ptr, int D, int page, long long heads, int box, bool half) {
+// [z, y, D] with 64 dims x rows of y x depth of z a box, 128-byte swizzle; boxes past the end read zeros
+bool make_map(CUtensorMap *map, const void *ptr, int D, long long y, long long z, int rows, int depth, bool half) {
   auto fn = encode_fn();
   if (!fn) return false;
-  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)page, (cuuint64_t)heads};
-  const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)D * 2 * page};
-  const cuuint32_t boxes[3] = {64, (cuuint32_t)box, 1}, es[3] = {1, 1, 1};
+  const cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)y, (cuuint64_t)z};
+  const cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)D * 2 * y};
+  const cuuint32_t boxes[3] = {64, (cuuint32_t)rows, (cuuint32_t)depth}, es[3] = {1, 1, 1};
   return fn(map, half ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void *>(ptr),
             dims, strides, boxes, es, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <class T, int D>
-cudaError_t launch(const TreeArgs &a, bool pdl, cudaStream_t st) {
-  auto kernel = tree_tc_kernel<T, D>;
+template <class T, int D, int PIPE>
+cudaError_t launch(const TreeArgs &a, int blocks, bool pdl, cudaStream_t st) {
+  using L = TcShape<D, PIPE>;
+  auto kernel = tree_tc_kernel<T, D, PIPE>;
   static std::atomic<int> attr_set[64];  // the shared-memory opt-in, once per device
   int dev = 0;
   if (const cudaError_t e = cudaGetDevice(&dev)) return e;
   if (dev < 64 && !attr_set[dev].load(std::memory_order_acquire)) {
-    if (const cudaError_t e =
-            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TcShape<D>::SMEM))
+    if (const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, L::SMEM))
       return e;
     attr_set[dev].store(1, std::memory_order_release);
   }
   int box = TA_KEYS;  // rows of a TMA box: the largest power of two up to a tile that divides the page
   while (a.page % box) box /= 2;
-  CUtensorMap mk, mv;
+  const int tpt = TT_ROWS / a.G;  // queries per row tile: whole ones, so that a box of the query map is a row tile
+  CUtensorMap mq, mk, mv;
   const bool half = !std::is_same<T, bf16>::value;
   const long long heads = (long long)a.num_pages * a.NKV;
-  if (!make_map(&mk, a.kc, D, a.page, heads, box, half) || !make_map(&mv, a.vc, D, a.page, heads, box, half))
+  if (!make_map(&mq, a.q, D, a.NQ, a.N, a.G, tpt, half) || !make_map(&mk, a.kc, D, a.page, heads, box, 1, half) ||
+      !make_map(&mv, a.vc, D, a.page, heads, box, 1, half))
     return cudaErrorNotSupported;
-  const int row_tiles = (a.max_q * a.G + TT_ROWS - 1) / TT_ROWS;
   cudaLaunchAttribute attr;
-  cudaLaunchConfig_t cfg = pdl_config(dim3(row_tiles * a.NKV * a.B, a.S), dim3(TT_THREADS), pdl, st, &attr);
-  cfg.dynamicSmemBytes = TcShape<D>::SMEM;
-  return cudaLaunchKernelEx(&cfg, kernel, mk, mv, a, row_tiles, box);
+  cudaLaunchConfig_t cfg = pdl_config(dim3(blocks), dim3(L::THREADS), pdl, st, &attr);
+  cfg.dynamicSmemBytes = L::SMEM;
+  return cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, a, box, tpt);
+}
+template <class T, int D>
+cudaError_t launch(const TreeArgs &a, bool pdl, cudaStream_t st) {
+  // Up to 128 rows a request: one row tile a block, two blocks an SM. More: two row tiles a block (they share the K and
+  // V tiles), one block an SM.
+  if (a.max_q <= TT_ROWS / a.G) return launch<T, D, 1>(a, 2 * device_sm_count(), pdl, st);
+  return launch<T, D, 2>(a, device_sm_count(), pdl, st);
 }
 
 }  // namespace
