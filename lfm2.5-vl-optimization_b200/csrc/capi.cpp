@@ -449,6 +449,7 @@ int lfm2q_qk_norm_rope_kv_paged(const uint16_t *qkv, int64_t row_stride, const u
   REQUIRE(N >= 0 && NQ > 0 && NKV > 0 && num_pages > 0 && page > 0,
           "qkv [N, (NQ + 2 NKV) * D], kc / vc [num_pages, NKV, page, D]: need N >= 0 and the others > 0");
   REQUIRE((long long)NQ + 2ll * NKV <= 65536, "NQ + 2 NKV must be <= 65536");
+  REQUIRE((long long)num_pages * page <= 0xffffffffll, "num_pages * page must be < 2^32");
   REQUIRE(rot_dim > 0 && rot_dim <= D && rot_dim % 16 == 0, "rot_dim must be a multiple of 16 in [16, D]");
   REQUIRE(row_stride >= ((long long)NQ + 2ll * NKV) * D && row_stride % 8 == 0,
           "qkv rows: the stride must be a multiple of 8 and hold (NQ + 2 NKV) * D");

@@ -18,9 +18,14 @@ namespace {
 
 // ------------------------------------------------------------------ kv_slots
 // need_b pages and tok_b tokens of a valid request; granted while the running sums (over all valid requests, in
-// order) stay within the free pages and the token capacity. One block: the scans run over 1024 requests at a time,
-// the page moves one warp a request. The kernel is latency: a few dependent loads and three block scans.
-constexpr int SL_T = 1024;
+// order) stay within the free pages and the token capacity. One block: the scans run over a block's worth of requests at
+// a time, the page moves one warp a request. The kernel is latency, a chain of dependent loads (lengths, free pages,
+// table) and barriers, so: the second scan (offsets without the refused requests) and the one of returned pages run only
+// where there are such, the search for a token's request runs in shared memory, and a small batch takes a small block.
+// Sums saturate at 2^30 (every limit is lower), so 32 bits hold them.
+constexpr uint32_t SL_MAX = 1u << 30;
+constexpr int SL_BIG = 1024;     // threads for batches of more than 256 requests
+constexpr int SL_FILL = 4096;    // token rows that the block fills itself
 
 struct SlotArgs {
   const int *lens, *want;
@@ -28,118 +33,112 @@ struct SlotArgs {
   int *got, *cu;
   int64_t *positions, *slots;
   int B, width, pool, page;
-  long long capacity;
+  int capacity;
 };
 
-// inclusive scans of a, b and c over the block's 1024 threads (64-bit: sums of wild requests do not wrap)
-__device__ __forceinline__ void block_scan3(long long &a, long long &b, long long &c, long long (*part)[3]) {
+__device__ __forceinline__ uint32_t sat_add(uint32_t a, uint32_t b) { return min(a + b, SL_MAX); }
+// inclusive saturating scans of two values over a block of SL_T threads, and their totals; part: [SL_T / 32]
+template <int SL_T>
+__device__ __forceinline__ void block_scan2(uint32_t &a, uint32_t &b, uint2 &total, uint2 *part) {
   const int lane = threadIdx.x & 31, wp = threadIdx.x >> 5;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const long long a2 = __shfl_up_sync(0xffffffffu, a, o), b2 = __shfl_up_sync(0xffffffffu, b, o),
-                    c2 = __shfl_up_sync(0xffffffffu, c, o);
+    const uint32_t a2 = __shfl_up_sync(0xffffffffu, a, o), b2 = __shfl_up_sync(0xffffffffu, b, o);
     if (lane >= o) {
-      a += a2;
-      b += b2;
-      c += c2;
+      a = sat_add(a, a2);
+      b = sat_add(b, b2);
     }
   }
   __syncthreads();  // part's last readers
-  if (lane == 31) {
-    part[wp][0] = a;
-    part[wp][1] = b;
-    part[wp][2] = c;
-  }
+  if (lane == 31) part[wp] = make_uint2(a, b);
   __syncthreads();
-  if (wp == 0) {
-    long long x = part[lane][0], y = part[lane][1], z = part[lane][2];
+  uint32_t ta = 0, tb = 0;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const long long x2 = __shfl_up_sync(0xffffffffu, x, o), y2 = __shfl_up_sync(0xffffffffu, y, o),
-                      z2 = __shfl_up_sync(0xffffffffu, z, o);
-      if (lane >= o) {
-        x += x2;
-        y += y2;
-        z += z2;
-      }
+  for (int w = 0; w < SL_T / 32; ++w) {
+    if (w == wp) {
+      a = sat_add(a, ta);
+      b = sat_add(b, tb);
     }
-    part[lane][0] = x;
-    part[lane][1] = y;
-    part[lane][2] = z;
+    ta = sat_add(ta, part[w].x);
+    tb = sat_add(tb, part[w].y);
   }
-  __syncthreads();
-  if (wp > 0) {
-    a += part[wp - 1][0];
-    b += part[wp - 1][1];
-    c += part[wp - 1][2];
-  }
+  total = make_uint2(ta, tb);
 }
 
-__device__ __forceinline__ int pages_of(long long len, int page) { return (int)((len + page - 1) / page); }
+__device__ __forceinline__ int pages_of(int len, int page) { return (int)(((unsigned)len + page - 1) / (unsigned)page); }
 
-// token i of the batch: its request is the last b with cu[b] <= i (requests without tokens share an offset with the
-// next one, and the last of them is the one that holds i)
-__device__ __forceinline__ void fill_slot(const SlotArgs &a, long long i) {
+// Token i of the batch: its request is the last b with cu[b] <= i (requests without tokens share an offset with the next
+// one, and the last of them is the one that holds i). SHARED: cu and lens are copies in shared memory.
+template <bool SHARED>
+__device__ __forceinline__ void fill_slot(const SlotArgs &a, const int *cu, const int *lens, int i) {
   int lo = 0, hi = a.B;  // cu[lo] <= i < cu[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
-    if (__ldcg(a.cu + mid) <= i) lo = mid;
+    if ((SHARED ? cu[mid] : __ldcg(cu + mid)) <= i) lo = mid;
     else hi = mid;
   }
-  const long long pos = __ldcg(a.lens + lo) + (i - __ldcg(a.cu + lo));
+  const unsigned pos = SHARED ? lens[lo] + (i - cu[lo]) : __ldcg(lens + lo) + (i - __ldcg(cu + lo));
+  const unsigned pg = pos / (unsigned)a.page;
   a.positions[i] = pos;
-  a.slots[i] = (long long)__ldcg(a.table + (size_t)lo * a.width + pos / a.page) * a.page + pos % a.page;
+  a.slots[i] = (long long)__ldcg(a.table + (size_t)lo * a.width + pg) * a.page + (pos - pg * a.page);
 }
 
-template <bool FILL>
+template <int SL_T>
 __global__ void __launch_bounds__(SL_T) kv_slots_kernel(const SlotArgs a) {
-  __shared__ long long part[32][3];
+  __shared__ uint2 part[SL_T / 32];
   __shared__ int s_old[SL_T], s_need[SL_T], s_ret[SL_T];  // old page count, pages taken / returned
-  __shared__ int s_need_off[SL_T], s_ret_off[SL_T];
+  __shared__ int s_need_off[SL_T], s_ret_off[SL_T], s_cu[SL_T], s_len[SL_T];
   pdl_trigger();
   pdl_wait();
   const int t = threadIdx.x, lane = t & 31, wp = t >> 5;
-  const long long room = (long long)a.width * a.page;
-  const int n0 = min(max(__ldcg(a.n_free), 0), a.pool);
-  // pass 1: what is granted. Offsets of the granted requests come out of a second scan, since a refused one takes
-  // nothing.
-  long long need_run = 0, tok_run = 0, tok_off = 0, P = 0, R = 0;
-  for (int b0 = 0; b0 < a.B; b0 += SL_T) {
+  const int room = a.width * a.page;  // <= 2^30
+  const bool one = a.B <= SL_T;       // one chunk: everything stays in shared memory
+  uint32_t need_run = 0, tok_run = 0, tok_off = 0, P = 0, R = 0, n0 = 0;
+  // pass 1: what is granted, and the offsets of the granted
+  for (int b0 = 0; b0 == 0 || b0 < a.B; b0 += SL_T) {
     const int b = b0 + t;
-    long long len = 0, want = 0, need = 0, tok = 0, zero = 0;
-    bool ok = false;
+    int len = 0, want = 0;
     if (b < a.B) {
       len = __ldcg(a.lens + b);
       want = __ldcg(a.want + b);
-      ok = len >= 0 && want >= 0 && len <= room && want <= room;
-      if (ok) {
-        need = max(0, pages_of(want, a.page) - pages_of(len, a.page));
-        tok = max(0ll, want - len);
-      }
     }
-    long long ns = need, ts = tok;
-    block_scan3(ns, ts, zero, part);
-    ok = ok && (need == 0 || need_run + ns <= n0) && (tok == 0 || tok_run + ts <= a.capacity);
-    need_run += part[31][0];
-    tok_run += part[31][1];
-    if (!ok) need = tok = 0;
-    long long ret = ok ? max(0, pages_of(len, a.page) - pages_of(want, a.page)) : 0;
-    long long gn = need, gt = tok, gr = ret;
-    block_scan3(gn, gt, gr, part);
+    if (b0 == 0) n0 = min(max(__ldcg(a.n_free), 0), a.pool);
+    bool ok = b < a.B && len >= 0 && want >= 0 && len <= room && want <= room;
+    const int old = ok ? pages_of(len, a.page) : 0, now = ok ? pages_of(want, a.page) : 0;
+    uint32_t need = ok ? max(0, now - old) : 0, tok = ok ? max(0, want - len) : 0;
+    uint32_t ns = need, ts = tok;
+    uint2 total;
+    block_scan2<SL_T>(ns, ts, total, part);
+    const bool fits = (need == 0 || sat_add(need_run, ns) <= n0) && (tok == 0 || sat_add(tok_run, ts) <= (uint32_t)a.capacity);
+    need_run = sat_add(need_run, total.x);
+    tok_run = sat_add(tok_run, total.y);
+    if (__syncthreads_or(ok && !fits)) {  // without the refused
+      ok = ok && fits;
+      if (!ok) need = tok = 0;
+      ns = need;
+      ts = tok;
+      block_scan2<SL_T>(ns, ts, total, part);
+    }
+    uint32_t ret = ok ? max(0, old - now) : 0, rs = ret, zero = 0;
+    uint2 rtotal = make_uint2(0, 0);
+    if (__syncthreads_or(ret)) block_scan2<SL_T>(rs, zero, rtotal, part);
+    const int at = (int)(tok_off + ts - tok);
     if (b < a.B) {
-      a.got[b] = (int)(ok ? want : len);
-      a.cu[b] = (int)(tok_off + gt - tok);
+      a.got[b] = ok ? want : len;
+      a.cu[b] = at;
     }
-    if (a.B <= SL_T) {  // one chunk: the offsets stay where the page moves read them
-      s_old[t] = ok ? pages_of(len, a.page) : 0;
+    if (one) {
+      s_old[t] = old;
       s_need[t] = (int)need;
       s_ret[t] = (int)ret;
-      s_need_off[t] = (int)(gn - need);
-      s_ret_off[t] = (int)(gr - ret);
+      s_need_off[t] = (int)(ns - need);
+      s_ret_off[t] = (int)(rs - ret);
+      s_cu[t] = at;
+      s_len[t] = len;
     }
-    P += part[31][0];
-    tok_off += part[31][1];
-    R += part[31][2];
+    P += total.x;
+    tok_off += total.y;
+    R += rtotal.x;
   }
   if (t == 0) a.cu[a.B] = (int)tok_off;
   __syncthreads();
@@ -148,9 +147,9 @@ __global__ void __launch_bounds__(SL_T) kv_slots_kernel(const SlotArgs a) {
   // ones were read from) returned pages
   for (int take = 1; take >= 0; --take) {
     if ((take ? P : R) == 0) continue;
-    long long off_run = 0;
+    uint32_t off_run = 0;
     for (int b0 = 0; b0 < a.B; b0 += SL_T) {
-      if (a.B > SL_T) {  // several chunks: a request's moves follow from lens and got
+      if (!one) {  // several chunks: a request's moves follow from lens and got
         const int b = b0 + t;
         int old = 0, moves = 0;
         if (b < a.B) {
@@ -160,12 +159,13 @@ __global__ void __launch_bounds__(SL_T) kv_slots_kernel(const SlotArgs a) {
             moves = max(0, take ? pages_of(got, a.page) - old : old - pages_of(got, a.page));
           }
         }
-        long long m = moves, z0 = 0, z1 = 0;
-        block_scan3(m, z0, z1, part);
+        uint32_t m = moves, z = 0;
+        uint2 total;
+        block_scan2<SL_T>(m, z, total, part);
         s_old[t] = old;
         (take ? s_need : s_ret)[t] = moves;
         (take ? s_need_off : s_ret_off)[t] = (int)(off_run + m - moves);
-        off_run += part[31][0];
+        off_run += total.x;
         __syncthreads();
       }
       const int nb = min(SL_T, a.B - b0);
@@ -173,11 +173,11 @@ __global__ void __launch_bounds__(SL_T) kv_slots_kernel(const SlotArgs a) {
         int *row = a.table + (size_t)(b0 + r) * a.width;
         if (take) {
           for (int j = lane; j < s_need[r]; j += 32)
-            row[s_old[r] + j] = __ldcg(a.freelist + (n0 - 1 - (s_need_off[r] + j)));
+            row[s_old[r] + j] = __ldcg(a.freelist + ((int)n0 - 1 - (s_need_off[r] + j)));
         } else {
           const int keep = s_old[r] - s_ret[r];
           for (int j = lane; j < s_ret[r]; j += 32) {
-            const long long at = n0 - P + R - 1 - (s_ret_off[r] + j);
+            const long long at = (long long)n0 - P + R - 1 - (s_ret_off[r] + j);
             if (at >= 0 && at < a.pool) a.freelist[at] = __ldcg(row + keep + j);
             row[keep + j] = -1;
           }
@@ -186,19 +186,34 @@ __global__ void __launch_bounds__(SL_T) kv_slots_kernel(const SlotArgs a) {
       __syncthreads();
     }
   }
-  if (t == 0) a.n_free[0] = (int)min((long long)a.pool, n0 - P + R);
-  if (FILL) {
-    __syncthreads();
-    const long long n = tok_off;
-    for (long long i = t; i < n; i += SL_T) fill_slot(a, i);
-  }
+  if (t == 0) a.n_free[0] = (int)min((long long)a.pool, (long long)n0 - P + R);
+  if (a.capacity <= SL_FILL)
+    for (int i = t; i < (int)tok_off; i += SL_T) {
+      if (one) fill_slot<true>(a, s_cu, s_len, i);
+      else fill_slot<false>(a, a.cu, a.lens, i);
+    }
 }
 
-__global__ void __launch_bounds__(256) kv_slots_fill_kernel(const SlotArgs a) {
+// Larger token capacities: a launch of its own. The offsets come into shared memory where they fit.
+constexpr int SF_T = 256, SF_MAX_B = 2048;
+__global__ void __launch_bounds__(SF_T) kv_slots_fill_kernel(const SlotArgs a) {
+  __shared__ int s_cu[SF_MAX_B], s_len[SF_MAX_B];
   pdl_trigger();
   pdl_wait();
-  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-  if (i < __ldcg(a.cu + a.B)) fill_slot(a, i);
+  const int n = __ldcg(a.cu + a.B);
+  if ((long long)blockIdx.x * SF_T >= n) return;
+  const bool small = a.B <= SF_MAX_B;
+  if (small) {
+    for (int b = threadIdx.x; b < a.B; b += SF_T) {
+      s_cu[b] = __ldcg(a.cu + b);
+      s_len[b] = __ldcg(a.lens + b);
+    }
+    __syncthreads();
+  }
+  for (long long i = (long long)blockIdx.x * SF_T + threadIdx.x; i < n; i += (long long)gridDim.x * SF_T) {
+    if (small) fill_slot<true>(a, s_cu, s_len, (int)i);
+    else fill_slot<false>(a, a.cu, a.lens, (int)i);
+  }
 }
 
 // ------------------------------------------------------------------ qk_norm_rope_kv_paged
@@ -233,11 +248,19 @@ struct RopeArgs {
 // in the same lane. Everything in fp32 and rounded once; the angle positions[n] * inv_freq[i] is formed and reduced
 // in fp64 (exact product, then off by about n_turns * 2^-52): in fp32 a position of 10^6 would lose the angle's
 // fourth digit.
-constexpr int RP_T = 256;
-constexpr int RP_UN = 4;  // pieces a thread keeps in flight
-template <class T, int D, bool INTER>
-__global__ void __launch_bounds__(RP_T) rope_paged_kernel(const RopeArgs a) {
-  constexpr int LPH = D / 8;  // lanes per head
+// Bounded by HBM at many tokens (16384 tokens, 32 + 8 + 8 heads of 128: 67 us, 6.0 TB/s, 91 % of the measured copy rate):
+// there 128 threads with 6 pieces each in flight and 8 blocks an SM were fastest (256 x 4: 78 us, 128 x 3: 75 us). Few
+// tokens are latency: 384 threads with 2 pieces each (one token: 2.2 us against 3.4).
+struct RopeMany {
+  static constexpr int T = 128, UN = 6, BLOCKS = 8;
+};
+struct RopeFew {
+  static constexpr int T = 384, UN = 2, BLOCKS = 4;
+};
+template <class T, int D, bool INTER, class SHAPE>
+__global__ void __launch_bounds__(SHAPE::T, SHAPE::BLOCKS) rope_paged_kernel(const RopeArgs a) {
+  constexpr int RP_T = SHAPE::T, RP_UN = SHAPE::UN;  // pieces a thread keeps in flight
+  constexpr int LPH = D / 8;                         // lanes per head
   __shared__ float2 cs[D / 2];
   pdl_trigger();
   pdl_wait();
@@ -251,18 +274,19 @@ __global__ void __launch_bounds__(RP_T) rope_paged_kernel(const RopeArgs a) {
     if (t + u * RP_T < pieces) raw[u] = ld_cg16(src + t + u * RP_T);
   const long long slot = __ldcg(reinterpret_cast<const long long *>(a.slots) + n);
   if (t < a.rot / 2) {
-    const double turn = 6.283185307179586476925;
-    const double ang = (double)__ldcg(reinterpret_cast<const long long *>(a.positions) + n) * (double)__ldg(a.inv_freq + t);
-    const float r = (float)fma(-rint(ang * (1.0 / turn)), turn, ang);
+    // in turns: the fraction keeps 2^-25 of one after its rounding to fp32
+    const double turns = (double)__ldcg(reinterpret_cast<const long long *>(a.positions) + n) * (double)__ldg(a.inv_freq + t) *
+                         0.15915494309189533577;
     float s, c;
-    sincosf(r, &s, &c);
+    sincospif(2.f * (float)(turns - rint(turns)), &s, &c);
     cs[t] = make_float2(c * a.scaling, s * a.scaling);
   }
   __syncthreads();
   const bool cached = slot >= 0 && slot < a.cache_slots;
   T *krow = nullptr, *vrow = nullptr;
   if (cached) {
-    const size_t at = ((size_t)(slot / a.page) * a.NKV * a.page + (size_t)(slot % a.page)) * D;
+    const unsigned pg = (unsigned)slot / (unsigned)a.page;  // (fewer than 2^32 slots: a cache of 2^38 elements)
+    const size_t at = ((size_t)pg * a.NKV * a.page + ((unsigned)slot - pg * a.page)) * D;
     krow = reinterpret_cast<T *>(a.kc) + at;
     vrow = reinterpret_cast<T *>(a.vc) + at;
   }
@@ -277,10 +301,9 @@ __global__ void __launch_bounds__(RP_T) rope_paged_kernel(const RopeArgs a) {
       if (p0 != t && live) raw[u] = ld_cg16(src + p);
       const int head = p / LPH, sub = p % LPH;
       const uint4 rv = live ? raw[u] : make_uint4(0, 0, 0, 0);
-      if (head >= a.NQ + a.NKV || !live) {
-        // values pass unchanged; the shuffles below need every lane of a warp that still holds q or k pieces
-        if (live && cached) *reinterpret_cast<uint4 *>(vrow + (head - a.NQ - a.NKV) * head_step + 8 * sub) = rv;
-      }
+      if (head >= a.NQ + a.NKV && live && cached)  // values pass unchanged
+        *reinterpret_cast<uint4 *>(vrow + (head - a.NQ - a.NKV) * head_step + 8 * sub) = rv;
+      if (__all_sync(0xffffffffu, head >= a.NQ + a.NKV)) continue;  // (the shuffles below need every lane otherwise)
       float x[8];
       {
         const uint32_t w[4] = {rv.x, rv.y, rv.z, rv.w};
@@ -348,17 +371,15 @@ __global__ void __launch_bounds__(RP_T) rope_paged_kernel(const RopeArgs a) {
 cudaError_t launch_kv_slots(const int *lens, const int *want, int *table, int *freelist, int *n_free, int *got, int *cu,
                             int64_t *positions, int64_t *slots, int B, int width, int pool, int page,
                             long long capacity, bool pdl, cudaStream_t st) {
-  const SlotArgs a{lens, want, table, freelist, n_free, got, cu, positions, slots, B, width, pool, page, capacity};
+  const SlotArgs a{lens, want, table, freelist, n_free, got, cu, positions, slots, B, width, pool, page, (int)capacity};
   cudaLaunchAttribute attr;
-  // Up to 4096 token slots the one block fills them itself; more get a launch of their own with a block per 256.
-  if (capacity <= 4 * SL_T) {
-    const cudaLaunchConfig_t cfg = pdl_config(dim3(1), dim3(SL_T), pdl, st, &attr);
-    return cudaLaunchKernelEx(&cfg, kv_slots_kernel<true>, a);
-  }
-  cudaLaunchConfig_t cfg = pdl_config(dim3(1), dim3(SL_T), pdl, st, &attr);
-  if (const cudaError_t e = cudaLaunchKernelEx(&cfg, kv_slots_kernel<false>, a)) return e;
-  cfg.gridDim = dim3((unsigned)((capacity + 255) / 256));
-  cfg.blockDim = dim3(256);
+  cudaLaunchConfig_t cfg = pdl_config(dim3(1), dim3(B <= 256 ? 256 : SL_BIG), pdl, st, &attr);
+  if (const cudaError_t e = B <= 256 ? cudaLaunchKernelEx(&cfg, kv_slots_kernel<256>, a)
+                                     : cudaLaunchKernelEx(&cfg, kv_slots_kernel<SL_BIG>, a))
+    return e;
+  if (capacity <= SL_FILL) return cudaSuccess;
+  cfg.gridDim = dim3((unsigned)std::min<long long>((capacity + SF_T - 1) / SF_T, 4LL * device_sm_count()));
+  cfg.blockDim = dim3(SF_T);
   return cudaLaunchKernelEx(&cfg, kv_slots_fill_kernel, a);
 }
 
@@ -369,15 +390,20 @@ cudaError_t launch_qk_norm_rope_kv_paged(const void *qkv, long long row_stride, 
                                          bool pdl, cudaStream_t st) {
   const RopeArgs a{qkv, qw, kw, inv_freq, positions, slots, q_out, kc, vc, row_stride, num_pages * page,
                    N, NQ, NKV, page, rot, scaling, eps};
-  cudaLaunchAttribute attr;
-  const cudaLaunchConfig_t cfg = pdl_config(dim3(N), dim3(RP_T), pdl, st, &attr);
-  auto go = [&](auto kernel) { return cudaLaunchKernelEx(&cfg, kernel, a); };
+  auto go = [&](auto many, auto few) {
+    const bool is_few = N <= 2 * device_sm_count();
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = pdl_config(dim3(N), dim3(is_few ? RopeFew::T : RopeMany::T), pdl, st, &attr);
+    return cudaLaunchKernelEx(&cfg, is_few ? few : many, a);
+  };
+#define LFM2Q_ROPE(T, D, I) go(rope_paged_kernel<T, D, I, RopeMany>, rope_paged_kernel<T, D, I, RopeFew>)
   if (half) {
-    if (D == 64) return interleaved ? go(rope_paged_kernel<__half, 64, true>) : go(rope_paged_kernel<__half, 64, false>);
-    return interleaved ? go(rope_paged_kernel<__half, 128, true>) : go(rope_paged_kernel<__half, 128, false>);
+    if (D == 64) return interleaved ? LFM2Q_ROPE(__half, 64, true) : LFM2Q_ROPE(__half, 64, false);
+    return interleaved ? LFM2Q_ROPE(__half, 128, true) : LFM2Q_ROPE(__half, 128, false);
   }
-  if (D == 64) return interleaved ? go(rope_paged_kernel<bf16, 64, true>) : go(rope_paged_kernel<bf16, 64, false>);
-  return interleaved ? go(rope_paged_kernel<bf16, 128, true>) : go(rope_paged_kernel<bf16, 128, false>);
+  if (D == 64) return interleaved ? LFM2Q_ROPE(bf16, 64, true) : LFM2Q_ROPE(bf16, 64, false);
+  return interleaved ? LFM2Q_ROPE(bf16, 128, true) : LFM2Q_ROPE(bf16, 128, false);
+#undef LFM2Q_ROPE
 }
 
 }  // namespace lfm2q
