@@ -406,6 +406,7 @@ __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
 
 // One warp per (query, head): the parts joined in order. A row of one part has been written by its block.
 constexpr int TC_WARPS = 4;
+constexpr int UNR = 8;
 template <class T, int D>
 __global__ void __launch_bounds__(32 * TC_WARPS) tree_combine_kernel(const TreeArgs a) {
   constexpr int DPL = D / 32;  // dims per lane
@@ -417,25 +418,38 @@ __global__ void __launch_bounds__(32 * TC_WARPS) tree_combine_kernel(const TreeA
   if (i >= rq.T) return;
   const size_t row = (size_t)(rq.n0 + i) * a.NQ + h;
   const float *info = ws_row(a, D, row);
-  const int parts = __ldcg(reinterpret_cast<const int *>(info));
+  // one load brings the number of parts (lane 0) and up to 31 parts' logarithms (lane 1 + part)
+  const float first = lane <= a.S ? __ldcg(info + lane) : -INFINITY;
+  const int parts = __shfl_sync(0xffffffffu, __float_as_int(first), 0);
   if (parts <= 1) return;
-  float M = -INFINITY;
-  for (int s = lane; s < parts; s += 32) M = fmaxf(M, __ldcg(info + 1 + s));
+  float M = lane > 0 && lane <= parts ? first : -INFINITY;
+  for (int s = 31 + lane; s < parts; s += 32) M = fmaxf(M, __ldcg(info + 1 + s));
   M = warp_max(M);
   const float ms = M == -INFINITY ? 0.f : M;
   float L = 0.f, acc[DPL];
 #pragma unroll
   for (int j = 0; j < DPL; ++j) acc[j] = 0.f;
-#pragma unroll 4
-  for (int s = 0; s < parts; ++s) {
-    const float c = ex2(__ldcg(info + 1 + s) - ms);
-    const float *p = ws_acc(a, D, s, row) + DPL * lane;
-    L += c;
+  for (int s0 = 0; s0 < parts; s0 += UNR) {  // UNR parts in flight
+    float2 v[UNR][DPL / 2];
 #pragma unroll
-    for (int j = 0; j < DPL; j += 2) {
-      const float2 v = __ldcg(reinterpret_cast<const float2 *>(p + j));
-      acc[j] += v.x * c;
-      acc[j + 1] += v.y * c;
+    for (int u = 0; u < UNR; ++u) {
+      const float *p = ws_acc(a, D, min(s0 + u, parts - 1), row) + DPL * lane;
+#pragma unroll
+      for (int j = 0; j < DPL; j += 2) v[u][j / 2] = __ldcg(reinterpret_cast<const float2 *>(p + j));
+    }
+#pragma unroll
+    for (int u = 0; u < UNR; ++u) {
+      const int s = s0 + u;
+      const float lse = s < 31 ? __shfl_sync(0xffffffffu, first, (s + 1) & 31) : s < parts ? __ldcg(info + 1 + s) : 0.f;
+      if (s < parts) {
+        const float c = ex2(lse - ms);
+        L += c;
+#pragma unroll
+        for (int j = 0; j < DPL; j += 2) {
+          acc[j] += v[u][j / 2].x * c;
+          acc[j + 1] += v[u][j / 2].y * c;
+        }
+      }
     }
   }
   const float inv = L == 0.f ? 0.f : 1.f / L;

@@ -56,6 +56,7 @@ struct TreeArgs {
 // the table.
 struct Request {
   int n0, T, ctx, len;
+  __device__ __forceinline__ Request() {}
   __device__ __forceinline__ Request(const TreeArgs &a, int b) {
     const int c0 = __ldcg(a.cu + b), c1 = __ldcg(a.cu + b + 1);
     n0 = min(max(c0, 0), a.N);
@@ -93,37 +94,54 @@ struct TreePlan {
   long long base;   // tiles before that request
   long long off;    // of the block's first tile within it
   long long count;  // tiles of the block
+  int r_n0, r_T, r_ctx, r_len;  // lane i: request i (of the first 32)
   static __device__ __forceinline__ int tiles(const Request &rq) { return (rq.len + TA_KEYS - 1) / TA_KEYS; }
   // what a unit of n tiles takes of the line
   static __device__ __forceinline__ int span(const TreeArgs &a, int n) { return a.S == 1 ? 1 : n + TA_UNIT_COST; }
   __device__ __forceinline__ int units(const TreeArgs &a, const Request &rq) const {
     return a.NKV * ((rq.T * a.G + rows - 1) / rows);
   }
-  __device__ __forceinline__ long long weight(const TreeArgs &a, int i, int &n) const {
+  __device__ __forceinline__ long long weight(const TreeArgs &a, const Request &rq, int &n) const {
     n = 0;
-    if (i >= a.B) return 0;
-    const Request rq(a, i);
     if (rq.T == 0) return 0;
     n = tiles(rq);
     return (long long)units(a, rq) * span(a, n);
+  }
+  // request i, for a whole warp: of the first 32 without another load
+  __device__ __forceinline__ Request request(const TreeArgs &a, int i) const {
+    if (i >= 32) return Request(a, i);
+    Request rq;
+    rq.n0 = __shfl_sync(0xffffffffu, r_n0, i);
+    rq.T = __shfl_sync(0xffffffffu, r_T, i);
+    rq.ctx = __shfl_sync(0xffffffffu, r_ctx, i);
+    rq.len = __shfl_sync(0xffffffffu, r_len, i);
+    return rq;
   }
   // For a whole warp: the stretch of block c of `blocks`.
   __device__ __forceinline__ TreePlan(const TreeArgs &a, int rows_, int blocks, int c) : rows(rows_), b(a.B), base(0) {
     const int lane = threadIdx.x & 31;
     int longest = 1;
     long long total = 0, first = 0;
+    r_n0 = r_T = r_ctx = r_len = 0;
 #pragma unroll 4
     for (int i = lane; i < a.B; i += 32) {
       int n;
-      const long long w = weight(a, i, n);
-      if (i == lane) first = w;
+      const Request rq(a, i);
+      const long long w = weight(a, rq, n);
+      if (i == lane) {
+        first = w;
+        r_n0 = rq.n0;
+        r_T = rq.T;
+        r_ctx = rq.ctx;
+        r_len = rq.len;
+      }
       total += w;
       longest = max(longest, n);
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
     longest = __reduce_max_sync(0xffffffffu, longest);
-    quota = (total + blocks - 1) / blocks;
+    quota = total < 0x7fff0000 ? ((int)total + blocks - 1) / blocks : (total + blocks - 1) / blocks;
     if (a.S > 1) quota = max(quota, (long long)((longest + a.S - 2) / (a.S - 1)));
     quota = max(quota, 1ll);
     const long long x0 = quota * c;
@@ -131,7 +149,7 @@ struct TreePlan {
     long long run = 0;
     for (int b0 = 0; count > 0 && b0 < a.B; b0 += 32) {
       int n;
-      const long long w = b0 == 0 ? first : weight(a, b0 + lane, n);
+      const long long w = b0 == 0 ? first : b0 + lane < a.B ? weight(a, Request(a, b0 + lane), n) : 0;
       long long s = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {

@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
       Segment g = {};
       int t1 = 0;
       while (left > 0 && b < a.B) {
-        const Request rq(a, b);
+        const Request rq = plan.request(a, b);
         const int units = plan.units(a, rq), n = plan.tiles(rq), span = plan.span(a, n);
         const long long w = (long long)units * span;
         if (off >= w) {
