@@ -420,7 +420,8 @@ __global__ void __launch_bounds__(32 * TC_WARPS) tree_combine_kernel(const TreeA
   const float *info = ws_row(a, D, row);
   // one load brings the number of parts (lane 0) and up to 31 parts' logarithms (lane 1 + part)
   const float first = lane <= a.S ? __ldcg(info + lane) : -INFINITY;
-  const int parts = __shfl_sync(0xffffffffu, __float_as_int(first), 0);
+  // (held to S: after a wait that gave up the words were never written)
+  const int parts = min(__shfl_sync(0xffffffffu, __float_as_int(first), 0), a.S);
   if (parts <= 1) return;
   float M = lane > 0 && lane <= parts ? first : -INFINITY;
   for (int s = 31 + lane; s < parts; s += 32) M = fmaxf(M, __ldcg(info + 1 + s));

@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
   if (warp == W_TMA) {
     // ---------------------------------------------------------------- segments, queries, K and V tiles
     const TreePlan plan(a, PIPE * tpt * a.G, gridDim.x, blockIdx.x);
-    const int boxes = TA_KEYS / box;
+    const int boxes = TA_KEYS / box, page_step = TA_KEYS / a.page, row_step = TA_KEYS % a.page;
     long long left = plan.count, off = plan.off, base = plan.base;
     int b = plan.b, st = 0, ph = 1;  // a fresh barrier passes a wait for the phase before its first
     uint32_t issued = 0, seg = 0;
@@ -298,20 +298,34 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
             tma_load_3d(sq + p * L::Q_BYTES + h * TT_ATOM, &tmQ, smem_addr(&q_full), 64 * h, g.kvh * a.G,
                         g.n0 + g.tok0 + p * tpt);
       }
+      // Page numbers come a tile ahead: their load takes as long as a tile (loaded where they were used, the loading warp
+      // bounded the kernel, 217 us where it is 170 now).
       const int *table = a.table + (size_t)g.b * a.width;
+      int idx[2], y[2], ahead[2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int i = lane + 32 * u, t = g.t0 + i * box;
+        idx[u] = t / a.page;
+        y[u] = t - idx[u] * a.page;
+        ahead[u] = i < boxes && t < t1 ? __ldcg(table + idx[u]) : -1;
+      }
       for (int n = 0; n < g.tiles; ++n, ++issued) {
         const int tile_at = g.t0 + n * TA_KEYS;
-        int pg[2], y[2] = {0, 0};
+        int pg[2], row[2];
         uint32_t mine = 0;
         unsigned long long keys = 0;  // of this lane's boxes
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int i = lane + 32 * u, t = tile_at + i * box;
-          pg[u] = -1;
-          if (i < boxes && t < t1) {
-            pg[u] = __ldcg(table + t / a.page);
-            y[u] = t % a.page;
+          pg[u] = ahead[u];
+          row[u] = y[u];
+          idx[u] += page_step;
+          y[u] += row_step;
+          if (y[u] >= a.page) {
+            y[u] -= a.page;
+            ++idx[u];
           }
+          ahead[u] = n + 1 < g.tiles && i < boxes && t + TA_KEYS < t1 ? __ldcg(table + idx[u]) : -1;
           if (pg[u] < 0 || pg[u] >= a.num_pages) {
             pg[u] = -1;
           } else {
@@ -336,14 +350,14 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
           if (pg[u] >= 0)
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
-              tma_load_3d(sk + st * L::KV_BYTES + h * TT_HALF + (lane + 32 * u) * box * 128, &tmK, bar, 64 * h, y[u],
+              tma_load_3d(sk + st * L::KV_BYTES + h * TT_HALF + (lane + 32 * u) * box * 128, &tmK, bar, 64 * h, row[u],
                           pg[u] * a.NKV + g.kvh);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
           if (pg[u] >= 0)
 #pragma unroll
             for (int h = 0; h < HALVES; ++h)
-              tma_load_3d(sv + st * L::KV_BYTES + h * TT_HALF + (lane + 32 * u) * box * 128, &tmV, bar, 64 * h, y[u],
+              tma_load_3d(sv + st * L::KV_BYTES + h * TT_HALF + (lane + 32 * u) * box * 128, &tmV, bar, 64 * h, row[u],
                           pg[u] * a.NKV + g.kvh);
         if (++st == STAGES) {
           st = 0;
