@@ -38,9 +38,10 @@ const char *lfm2q_version(void);
 /* 1 if the current device is an sm_100 part this library can launch on, else 0. */
 int lfm2q_device_supported(void);
 
-/* Reads (and with clear != 0 resets) the sticky device error words that the tcgen05 GEMMs and the decode attention
- * set when one of their bounded pipeline waits gives up (no other kernel of this library waits on anything).
- * Returns LFM2Q_OK or LFM2Q_ETIMEOUT. Synchronous (copies two ints from the device). Poll it after a batch of work
+/* Reads (and with clear != 0 resets) the sticky device error words that the tcgen05 GEMMs, the decode attention and the
+ * tree attention set when one of their bounded pipeline waits gives up (no other kernel of this library waits on
+ * anything but its own cluster's barriers). Returns LFM2Q_OK or LFM2Q_ETIMEOUT. Synchronous (copies three ints from the
+ * device). Poll it after a batch of work
  * whose outputs matter. */
 int lfm2q_check_device(int clear);
 
@@ -270,8 +271,10 @@ int lfm2q_qk_norm_rope_kv_paged(const uint16_t *qkv, int64_t row_stride, const u
  * = softmax(scale q.k) v; a query that sees nothing gives zeros. Rows outside the requests, and those past max_q of a
  * request, are left as they were. NQ = G NKV, G <= 64; D 64 or 128; scale > 0. A position whose page is outside
  * [0, num_pages), or past the table, is not seen.
- * S splits over the positions (lfm2q_tree_attention_splits suggests a number): with S > 1 ws fp32 [N, NQ, S, D + 2]
- * holds (m, l, acc[D]) of each (no value needs to be set before; concurrent calls need their own); S = 1 needs none. */
+ * The positions of a request are cut into at most S parts (lfm2q_tree_attention_splits suggests a number): with S > 1 ws,
+ * fp32, N * NQ * S * (D + 2) words, holds the parts' results until a second kernel joins them (no value needs to be set
+ * before; calls that may run at the same time need their own); S = 1 needs none. Results do not depend on what ws held;
+ * they depend on S and on the other requests of the call only by the order of fp32 sums. */
 int lfm2q_tree_attention(const uint16_t *q, const uint16_t *kc, const uint16_t *vc, const int32_t *table,
                          const int32_t *ctx, const int32_t *cu, const int64_t *mask, uint16_t *out, float *ws,
                          int dtype, int N, int B, int NQ, int NKV, int D, int num_pages, int page, int max_pages, int S,
@@ -284,9 +287,9 @@ int lfm2q_tree_attention_splits(int B, int NQ, int NKV, int D, int max_q, int ma
  * elements apart, any alignment of rows): temperature T > 0: w_i = e^((x_i - max) / T); in the order (x descending,
  * index ascending) the first top_k are kept (0 or less: all), of those the shortest prefix whose mass reaches top_p of
  * theirs (>= 1 or NaN: all; always at least one), of those w_i >= min_p (of the largest, 1). tok[b] = the first index
- * whose running kept mass, in index order, exceeds u[b] (in [0, 1)) times the kept mass. T <= 0 or NaN, a NaN among the
- * logits, or no finite one: the argmax, as lfm2q_argmax_next. A NULL temperature, top_k, top_p or min_p [B] is off
- * (temperature 1). Weights are summed as integers in steps of 2^-44 of the largest: the same token in any launch
+ * whose running kept mass, in index order, exceeds u[b] (in [0, 1), values outside held to it, a NaN to 0) times the kept
+ * mass. T <= 0 or NaN, a NaN among the logits, or none above -inf: the argmax, as lfm2q_argmax_next. A NULL temperature,
+ * top_k, top_p or min_p [B] is off (temperature 1). Weights are summed as integers in steps of 2^-44 of the largest: the same token in any launch
  * shape. pos[0] += 1 if pos is not NULL. V <= 262144. */
 int lfm2q_sample_next(const void *logits, int dtype, int64_t row_stride, const float *temperature, const int32_t *top_k,
                       const float *top_p, const float *min_p, const float *u, int64_t *tok, int64_t *pos, int B, int V,

@@ -709,8 +709,9 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
 
   // ---------------------------------------------------------------- where the cut lies: bins [b_lo, b_hi]
   int b_lo = SA_BINS, b_hi = -1;  // no cut: everything is "above"
-  // the exact histograms where the list would be too long, or the maximum is infinite (every block finds the same)
-  bool again = best == INFINITY;
+  // the exact histograms where the list would be too long, or where the bins and the branch-free weights would meet 0
+  // times infinity: an infinite maximum, a temperature near 0 (every block finds the same)
+  bool again = best == INFINITY || !(bins.scale < 1e30f);
   if ((use_k || use_p) && !again) {
     for (int v = w0 + lane; v < w1; v += 32) {
       const uint4 q = stage[v];

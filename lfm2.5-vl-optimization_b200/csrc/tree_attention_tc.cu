@@ -202,7 +202,6 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
   uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(tt_smem) + 1023) & ~uintptr_t(1023));
   const uint32_t sq = smem_addr(smem), sk = sq + PIPE * L::Q_BYTES, sv = sk + STAGES * L::KV_BYTES;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  pdl_trigger();
   if (threadIdx.x == 0) {
     for (int i = 0; i < STAGES; ++i) {
       mbar_init(smem_addr(&full[i]), 1);
@@ -236,6 +235,9 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
+  // The next kernel may start only now that this block has its tensor memory: one that took the SM's first would hold
+  // it until this grid ends.
+  pdl_trigger();
   pdl_wait();
 
   if (warp == W_TMA) {

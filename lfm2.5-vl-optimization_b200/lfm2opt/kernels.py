@@ -5,12 +5,15 @@ prebuilt sm_100a library liblfm2q.so instead of a JIT build.
                 gemm_i8, gemm_i8_q, gemm_w8, quant_rows, add_layernorm_q, add_rmsnorm_q, silu_mul_q,
                 plus gemm_i8_silu (W8A8 GEMM with the SiLU(w1) * w3 gate fused into its epilogue)
     ext()       the GEMV part of the reference's lfm2_decode extension (kernels/lfm2_decode.cpp:152-168):
-                gemv, gemv_epi, gemv_w4, set_pdl, set_gemv_impl, plus gemv_a8 (int8 tokens x int8 weights, exact int32)
+                gemv, gemv_epi, gemv_w4, set_pdl, set_gemv_impl, plus gemv_a8 (int8 tokens x int8 weights, exact int32);
+                its decode-step kernels add_rmsnorm, shortconv_step, qk_norm_rope_kv and decode_attention_split; and, with
+                no counterpart there, embed_rmsnorm, argmax_next and the operators of batches of requests over a paged
+                cache: kv_slots, qk_norm_rope_kv_paged, tree_attention, sample_next
 
 Argument names, meaning, in-place outputs and the RuntimeError messages of the shape checks follow the reference
 bindings (kernels/int8_gemm.cpp:20-141, kernels/lfm2_decode.cpp:30-150). Every op enqueues on PyTorch's current
-stream of the tensors' device and returns None. The decode extension's non-GEMV kernels (attention, RoPE, conv,
-norms) are not part of this library; reaching for them raises AttributeError.
+stream of the tensors' device and returns None. The decode extension's remaining kernels (the unsplit attention, the
+bf16 silu_mul, prefill) are not part of this library; reaching for them raises AttributeError.
 """
 
 import ctypes
@@ -603,9 +606,8 @@ class GemvChain:
 
 
 def check_device(clear=False):
-    """Raise RuntimeError if a bounded pipeline wait inside a tcgen05 GEMM or the decode attention gave up since the
-    last clear (the outputs of
-    that work are then invalid). Synchronises with the current device. clear: reset the word."""
+    """Raise RuntimeError if a bounded pipeline wait inside a tcgen05 GEMM, the decode attention or the tree attention
+    gave up since the last clear (the outputs of that work are then invalid). Synchronises with the current device. clear: reset the word."""
     st = _capi.lib().lfm2q_check_device(int(bool(clear)))
     if st != _capi.OK:
         raise RuntimeError(_capi.lib().lfm2q_last_error().decode() or f"lfm2q_check_device: status {st}")

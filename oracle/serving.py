@@ -102,7 +102,9 @@ def tree_attention_f64(q, kc, vc, table, ctx, cu, mask, scale, max_q=64):
 
 
 def sample_next_f64(logits, temperature, top_k, top_p, min_p, u):
-    """The token of one row: logits a numpy array (any float type), the rest Python numbers."""
+    """The token of one row: logits a numpy array (any float type), the rest Python numbers. Masses are counted in whole
+    steps of 2^-44 of the largest weight, as the operator defines them (a weight below half a step counts as none: only a
+    u of 1 or more, held to the last step of the mass, would tell)."""
     x = np.asarray(logits, np.float64)
     if np.isnan(x).any():
         return int(np.flatnonzero(np.isnan(x))[0])
@@ -114,13 +116,15 @@ def sample_next_f64(logits, temperature, top_k, top_p, min_p, u):
     with np.errstate(invalid="ignore", over="ignore"):
         w = np.where(x == x.max(), 1.0, np.exp((x - x.max()) / temperature))
     w[x == -np.inf] = 0.0
+    least = min(min_p, 1.0) if min_p > 0 else 0.0
+    high, w = w >= least, np.rint(w * 2.0 ** 44)
     if top_p < 1:
         mass = w[order]
         before = np.cumsum(mass) - mass
         keep = before < max(top_p, 0.0) * mass.sum()
         keep[0] = True
         order = order[keep]
-    order = np.sort(order[w[order] >= (min(min_p, 1.0) if min_p > 0 else 0.0)])
+    order = np.sort(order[high[order]])
     run = np.cumsum(w[order])
     u = min(max(u, 0.0), 1.0) if u == u else 0.0
     return int(order[min(np.searchsorted(run, u * run[-1], side="right"), np.flatnonzero(w[order])[-1])])

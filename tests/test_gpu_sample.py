@@ -152,3 +152,29 @@ def test_capture_and_refusals(cuda_dev):
                         ((torch.zeros(3, (1 << 18) + 1, device=cuda_dev), None, None, None, None, u, tok), "262144")):
         with pytest.raises(RuntimeError, match=match):
             K.sample_next(*args)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+def test_extreme_parameters(cuda_dev, dt):
+    """Temperatures next to zero and infinite ones, uniforms at and past their ends, spreads beyond every bin."""
+    g = torch.Generator().manual_seed(7)
+    base = 3 * torch.randn(2500, generator=g)
+    rows, p = [], dict(temperature=[], top_k=[], top_p=[], min_p=[], u=[])
+    for T in (1e-45, 1e-38, 1e-30, 1e-20, 1e-3, 1e20, 3e38, float("inf")):
+        for k, tp in ((0, 1.0), (0, 0.5), (40, 1.0), (40, 0.5), (2400, 0.999)):
+            for u in (0.0, 0.5, 1.0, 1.5, -1.0, float("nan")):
+                rows.append(base)
+                for n, v in zip(p, (T, k, tp, 0.0, u)):
+                    p[n].append(v)
+    x = torch.stack(rows).to(DT[dt])
+    assert draw(cuda_dev, x, **p) == want(x, **p)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-6, 0.01, 1.0, 30.0, 3000.0])
+def test_spreads(cuda_dev, scale):
+    """Cuts in distributions from flat (thousands of elements in a bin) to a single spike."""
+    g = torch.Generator().manual_seed(8)
+    x = scale * torch.randn(30, 20000, generator=g)
+    p = params(np.random.default_rng(8), 30)
+    p["temperature"] = [1.0] * 30
+    assert draw(cuda_dev, x, **p) == want(x, **p)

@@ -225,3 +225,70 @@ def test_refusals(cuda_dev):
                       (dict(ws=torch.empty(3, 8, 2, 64, device=cuda_dev)), "ws")):
         with pytest.raises(RuntimeError, match=match):
             call(**kw)
+
+
+@pytest.mark.parametrize("D,dt,T,S", [(64, "bf16", 3, 1), (64, "fp16", 40, 4), (128, "bf16", 9, 3), (128, "fp16", 64, 2),
+                                      (64, "bf16", 64, 1)])
+@pytest.mark.parametrize("order", ["growing", "falling", "jumping"])
+def test_maxima_that_move_along_the_cache(cuda_dev, D, dt, T, S, order):
+    """Scores whose maximum grows by more than 2^8 from tile to tile (the accumulator is rescaled in every one, the last
+    included), falls, or jumps."""
+    c = make(11, 8, 2, D, 16, [450, 130], [T, 2], dt)
+    direction = torch.randn(D, generator=torch.Generator().manual_seed(5))
+    direction /= direction.norm()
+    for b in range(2):
+        L = int(c["ctx"][b]) + (T if b == 0 else 2)
+        for t in range(L):
+            step = t // 16 if order == "growing" else -(t // 16) if order == "falling" else (t // 64) * 37 % 29
+            k = c["kc"][int(c["table"][b, t // 16]), :, t % 16]
+            k.copy_((0.2 * k.float() + 4.0 * step * direction).to(k.dtype))
+    c["q"] = (0.3 * c["q"].float() + 4.0 * direction).to(c["q"].dtype)
+    check(run(cuda_dev, c, S), reference(c), c)
+
+
+def test_more_parts_than_a_warp_has_lanes(cuda_dev):
+    c = make(12, 8, 2, 64, 64, [4500], [2], "bf16")  # 71 tiles
+    for S in (70, 40):
+        check(run(cuda_dev, c, S), reference(c), c)
+
+
+@pytest.mark.parametrize("page", [8, 24, 40, 5, 200])
+def test_page_sizes_that_tiles_straddle(cuda_dev, page):
+    for D, T in ((64, 6), (128, 40)):
+        c = make(page, 12, 3, D, page, [333, 64], [T, T], "fp16")
+        check(run(cuda_dev, c, 3), reference(c), c)
+
+
+def test_many_requests_with_and_without_queries(cuda_dev):
+    """More requests than a warp has lanes and blocks have stretches; some bring nothing."""
+    rng = np.random.default_rng(13)
+    ctx, T = rng.integers(0, 150, 300).tolist(), rng.integers(0, 4, 300).tolist()
+    c = make(13, 4, 2, 64, 16, ctx, T, "bf16")
+    for S in (1, 3):
+        check(run(cuda_dev, c, S), reference(c), c)
+
+
+def test_two_streams_at_once(cuda_dev):
+    """Calls with workspaces of their own on two streams, among other kernels that use tensor memory."""
+    from lfm2opt.kernels import check_device, int8_ext
+    cs = [make(20 + i, 32, 8, 64, 64, [700, 300], [16, 9], "bf16") for i in range(2)]
+    refs = [reference(c) for c in cs]
+    streams = [torch.cuda.Stream(cuda_dev) for _ in cs]
+    xq = torch.randint(-127, 128, (512, 1024), dtype=torch.int8, device=cuda_dev)
+    sx, y = torch.ones(512, device=cuda_dev), torch.empty(512, 512, dtype=torch.bfloat16, device=cuda_dev)
+    work = []
+    for c in cs:
+        d = {k: v.to(cuda_dev) for k, v in c.items() if torch.is_tensor(v)}
+        work.append((d, signed(c["mask"]).to(cuda_dev), torch.full_like(d["q"], float("nan")),
+                     torch.empty(25, 32, 6, 66, device=cuda_dev)))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for s, c, (d, m, out, ws) in zip(streams, cs, work):
+            with torch.cuda.stream(s):
+                ext().tree_attention(d["q"], d["kc"], d["vc"], d["table"], d["ctx"], d["cu"], m, out, ws, c["scale"], 16)
+        with torch.cuda.stream(streams[0]):
+            int8_ext().gemm_i8(xq, sx, xq, sx, None, y, False)
+    torch.cuda.synchronize()
+    for c, ref, (_, _, out, _) in zip(cs, refs, work):
+        check(out, ref, c)
+    check_device()
