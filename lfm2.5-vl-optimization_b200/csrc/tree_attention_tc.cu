@@ -493,6 +493,28 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
               if (!((v1 >> j) & 1)) s1[j] = 0xff800000u;
             }
           }
+          // The probabilities with the maximum so far, while the tile's own is found (the exponentials and the
+          // comparisons run on different units); again where that has grown too much, which is rare.
+          const float2 c2 = make_float2(a.scale_log2, a.scale_log2);
+          uint32_t p[32];
+          float sum;
+          auto probabilities = [&]() {
+            const float ms = m == -INFINITY ? 0.f : m;
+            const float2 m2 = make_float2(-ms, -ms);
+            float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 x = ffma2(make_float2(__uint_as_float(s0[2 * j]), __uint_as_float(s0[2 * j + 1])), c2, m2);
+              const float2 y = ffma2(make_float2(__uint_as_float(s1[2 * j]), __uint_as_float(s1[2 * j + 1])), c2, m2);
+              const float2 e = make_float2(ex2(x.x), ex2(x.y)), f = make_float2(ex2(y.x), ex2(y.y));
+              p[j] = Pair<T>::pack(e.x, e.y);
+              p[16 + j] = Pair<T>::pack(f.x, f.y);
+              sum0 = fadd2(sum0, e);
+              sum1 = fadd2(sum1, f);
+            }
+            sum = (sum0.x + sum0.y) + (sum1.x + sum1.y);
+          };
+          probabilities();
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int j = 0; j < 32; ++j) mx[j & 3] = max3(mx[j & 3], __uint_as_float(s0[j]), __uint_as_float(s1[j]));
@@ -520,22 +542,9 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
                 tmem_st32(t_o + 32 * c, o);
               }
             }
+            probabilities();
           }
-          const float ms = m == -INFINITY ? 0.f : m;
-          const float2 c2 = make_float2(a.scale_log2, a.scale_log2), m2 = make_float2(-ms, -ms);
-          uint32_t p[32];
-          float2 sum0 = make_float2(0.f, 0.f), sum1 = sum0;
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const float2 x = ffma2(make_float2(__uint_as_float(s0[2 * j]), __uint_as_float(s0[2 * j + 1])), c2, m2);
-            const float2 y = ffma2(make_float2(__uint_as_float(s1[2 * j]), __uint_as_float(s1[2 * j + 1])), c2, m2);
-            const float2 e = make_float2(ex2(x.x), ex2(x.y)), f = make_float2(ex2(y.x), ex2(y.y));
-            p[j] = Pair<T>::pack(e.x, e.y);
-            p[16 + j] = Pair<T>::pack(f.x, f.y);
-            sum0 = fadd2(sum0, e);
-            sum1 = fadd2(sum1, f);
-          }
-          l += (sum0.x + sum0.y) + (sum1.x + sum1.y);
+          l += sum;
           tmem_st32(pbuf, p);
           // A key that a row does not see has p = 0, but 0 times an infinity or a NaN is a NaN: value rows that hold
           // one are zeroed in shared memory (stale ones of keys that do not exist, too), and drafts among them are
