@@ -880,10 +880,11 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
       s.above = x1;
     }
     cl.sync();
+    // -------------------------------------------------------------- block 0 brings it together; the others are done
+    int n = 0;
+    unsigned long long M = 0, A = 0;
     if (rank == 0) {
-      // ------------------------------------------------------------ block 0: sort the list, find the cut, draw
-      int n = 0, from[SA_MAX_C];
-      unsigned long long M = 0, A = 0;
+      int from[SA_MAX_C];
       {
         of_cluster(cl, &s, from, 0, [](const SampleShared *o) { return o->n_list; });
         ulonglong2 v[SA_MAX_C];
@@ -910,10 +911,25 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
           if (c == k) at = i - from[k];
         if (c > 0) s.f.key[i] = cl.map_shared_rank(&s, c)->f.key[at];
       }
+      if (t == 0) s.cut = 0;
+      __syncthreads();
+      if (use_p && !use_k) {  // does the cut lie in the list?
+        unsigned long long sum = 0, before, total;
+        for (int i = t; i < n; i += SA_T)
+          sum += Weigher::fixed(weigh(value_of<E>((uint32_t)(s.f.key[i] >> SA_IDX_BITS))));
+        block_offsets(warp_scan(sum), s.scan[0], before, total);
+        const unsigned long long need = mass_needed(par.top_p, M);
+        if (!(A < need && need <= A + total) && t < C) cl.map_shared_rank(&s, t)->again = 1;
+      }
+    }
+    cl.sync();
+    again = s.again != 0;
+    if (!again) {
+      if (rank != 0) return;
+      // ------------------------------------------------------------ sort the list, find the cut, draw
       int N2 = 64;
       while (N2 < n) N2 *= 2;
       for (int i = n + t; i < N2; i += SA_T) s.f.key[i] = 0;
-      if (t == 0) s.cut = 0;
       __syncthreads();
       sort_keys(s.f.key, N2);  // (no two keys are equal: their indexes differ)
       constexpr int EACH = SA_LIST / SA_T;  // consecutive list elements a thread
@@ -950,104 +966,100 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
         M = s.f.pre[limit - 1];
       }
       const unsigned long long need = use_p ? mass_needed(par.top_p, M) : 0;
-      bool fine = true;
       if (use_p) {
-        fine = A < need && need <= A + (n ? s.f.pre[n - 1] : 0);
         for (int i = t; i < limit; i += SA_T)
           if (A + (i ? s.f.pre[i - 1] : 0) < need && need <= A + s.f.pre[i]) s.cut = i + 1;
       } else if (t == 0) {
         s.cut = use_k ? limit : 0;
       }
       __syncthreads();
-      if (fine) {
-        const int cut = s.cut;
-        const unsigned long long last = cut ? s.f.key[cut - 1] : 0;  // kept: this key or a higher one (0: all)
-        // the kept list elements' weights to the warps that hold them
+      const int cut = s.cut;
+      const unsigned long long last = cut ? s.f.key[cut - 1] : 0;  // kept: this key or a higher one (0: all)
+      // the kept list elements' weights to the warps that hold them
 #pragma unroll
-        for (int j = 0; j < EACH; ++j) {
-          const int i = t * each + j;
-          if (j < each && i < cut && high[j]) {
-            const int e = (1 << SA_IDX_BITS) - 1 - (int)(s.f.key[i] & ((1 << SA_IDX_BITS) - 1));
-            const int v = (e + skew) / PER, b = v / per_block, bv = min(per_block, NV - b * per_block);
-            atomicAdd(&s.f.warps[b * SA_W + (v - b * per_block) / ((bv + SA_W - 1) / SA_W)], wl[j]);
-          }
+      for (int j = 0; j < EACH; ++j) {
+        const int i = t * each + j;
+        if (j < each && i < cut && high[j]) {
+          const int e = (1 << SA_IDX_BITS) - 1 - (int)(s.f.key[i] & ((1 << SA_IDX_BITS) - 1));
+          const int v = (e + skew) / PER, b = v / per_block, bv = min(per_block, NV - b * per_block);
+          atomicAdd(&s.f.warps[b * SA_W + (v - b * per_block) / ((bv + SA_W - 1) / SA_W)], wl[j]);
         }
-        __syncthreads();
-        if (wp == 0) {
-          // the warp segment in which the running mass passes the target
-          unsigned long long m[SA_MAX_C * SA_W / 32], mine = 0;
+      }
+      __syncthreads();
+      if (wp == 0) {
+        // the warp segment in which the running mass passes the target
+        unsigned long long m[SA_MAX_C * SA_W / 32], mine = 0;
 #pragma unroll
-          for (int j = 0; j < SA_MAX_C * SA_W / 32; ++j) {
-            const int i = lane * (SA_MAX_C * SA_W / 32) + j;
-            m[j] = i < C * SA_W ? s.f.warps[i] : 0;
-            mine += m[j];
+        for (int j = 0; j < SA_MAX_C * SA_W / 32; ++j) {
+          const int i = lane * (SA_MAX_C * SA_W / 32) + j;
+          m[j] = i < C * SA_W ? s.f.warps[i] : 0;
+          mine += m[j];
+        }
+        const unsigned long long inc = warp_scan(mine);
+        const unsigned long long target = target_of(par.u, __shfl_sync(0xffffffffu, inc, 31));
+        int seg = -1;
+        unsigned long long at = inc - mine, seg_before = 0;
+#pragma unroll
+        for (int j = 0; j < SA_MAX_C * SA_W / 32; ++j) {
+          if (at <= target && target < at + m[j]) {
+            seg = lane * (SA_MAX_C * SA_W / 32) + j;
+            seg_before = at;
           }
-          const unsigned long long inc = warp_scan(mine);
-          const unsigned long long target = target_of(par.u, __shfl_sync(0xffffffffu, inc, 31));
-          int seg = -1;
-          unsigned long long at = inc - mine, seg_before = 0;
-#pragma unroll
-          for (int j = 0; j < SA_MAX_C * SA_W / 32; ++j) {
-            if (at <= target && target < at + m[j]) {
-              seg = lane * (SA_MAX_C * SA_W / 32) + j;
-              seg_before = at;
-            }
-            at += m[j];
-          }
-          const int who = __ffs(__ballot_sync(0xffffffffu, seg >= 0)) - 1;
-          seg = __shfl_sync(0xffffffffu, seg, who);
-          at = __shfl_sync(0xffffffffu, seg_before, who);
-          // its pieces again, 32 at a time, in index order
-          const int b = seg / SA_W, bv0 = b * per_block, bv = min(per_block, NV - bv0), pw = (bv + SA_W - 1) / SA_W;
-          const uint4 *far = cl.map_shared_rank(stage, b);
-          const int s0 = min(seg % SA_W * pw, bv), s1 = min(s0 + pw, bv);
-          bool found = false;
-          for (int vb = s0; vb < s1 && !found; vb += 32) {
-            const int v = vb + lane, e0 = (bv0 + v) * PER - skew;
-            unsigned long long w[PER], mm = 0;
-            if (v < s1) {
-              const uint4 q = far[v];
-              const raw *qr = reinterpret_cast<const raw *>(&q);
-#pragma unroll
-              for (int j = 0; j < PER; ++j) {
-                const float f = E::up(qr[j]);
-                const unsigned long long key =
-                    (unsigned long long)key_of<E>(qr[j]) << SA_IDX_BITS | (unsigned)((1 << SA_IDX_BITS) - 1 - (e0 + j));
-                const double wd = weigh.finite(f);
-                w[j] = f == f && key >= last && wd >= mp ? Weigher::fixed(wd) : 0;
-                mm += w[j];
-              }
+          at += m[j];
+        }
+        const int who = __ffs(__ballot_sync(0xffffffffu, seg >= 0)) - 1;
+        seg = __shfl_sync(0xffffffffu, seg, who);
+        at = __shfl_sync(0xffffffffu, seg_before, who);
+        // its pieces again, 32 at a time, in index order
+        const int b = seg / SA_W, bv0 = b * per_block, bv = min(per_block, NV - bv0), pw = (bv + SA_W - 1) / SA_W;
+        const int s0 = min(seg % SA_W * pw, bv), s1 = min(s0 + pw, bv);
+        bool found = false;
+        for (int vb = s0; vb < s1 && !found; vb += 32) {
+          const int v = vb + lane, e0 = (bv0 + v) * PER - skew;
+          unsigned long long w[PER], mm = 0;
+          if (v < s1) {
+            uint4 q;
+            raw *qr = reinterpret_cast<raw *>(&q);
+            if (e0 >= 0 && e0 + PER <= a.V) {
+              q = ld_cg16(x + e0);
             } else {
 #pragma unroll
-              for (int j = 0; j < PER; ++j) w[j] = 0;
+              for (int j = 0; j < PER; ++j) qr[j] = e0 + j >= 0 && e0 + j < a.V ? __ldcg(x + e0 + j) : FILL;
             }
-            const unsigned long long ms = warp_scan(mm);
-            unsigned long long run2 = at + ms - mm;
 #pragma unroll
             for (int j = 0; j < PER; ++j) {
-              if (run2 <= target && target < run2 + w[j]) {
-                finish(e0 + j);
-                found = true;
-              }
-              run2 += w[j];
+              const float f = E::up(qr[j]);
+              const unsigned long long key =
+                  (unsigned long long)key_of<E>(qr[j]) << SA_IDX_BITS | (unsigned)((1 << SA_IDX_BITS) - 1 - (e0 + j));
+              const double wd = weigh.finite(f);
+              w[j] = f == f && key >= last && wd >= mp ? Weigher::fixed(wd) : 0;
+              mm += w[j];
             }
-            found = __any_sync(0xffffffffu, found);
-            at += __shfl_sync(0xffffffffu, ms, 31);
+          } else {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) w[j] = 0;
           }
+          const unsigned long long ms = warp_scan(mm);
+          unsigned long long run2 = at + ms - mm;
+#pragma unroll
+          for (int j = 0; j < PER; ++j) {
+            if (run2 <= target && target < run2 + w[j]) {
+              finish(e0 + j);
+              found = true;
+            }
+            run2 += w[j];
+          }
+          found = __any_sync(0xffffffffu, found);
+          at += __shfl_sync(0xffffffffu, ms, 31);
         }
-      } else if (t < C) {
-        cl.map_shared_rank(&s, t)->again = 1;  // the cut lies outside the list
       }
+      return;
     }
-    cl.sync();
-    again = s.again != 0;
   }
-  if (again) {
-    cl.sync();  // the counts have been read by every block
-    const int token = sample_exact<E>(cl, s, part, weigh, bins, par, a.V);
-    if (token >= 0) finish(token);
-    cl.sync();
-  }
+  cl.sync();  // the counts have been read by every block
+  const int token = sample_exact<E>(cl, s, part, weigh, bins, par, a.V);
+  if (token >= 0) finish(token);
+  cl.sync();
 }
 
 template <class E>
