@@ -1007,51 +1007,55 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
           }
           at += m[j];
         }
-        const int who = __ffs(__ballot_sync(0xffffffffu, seg >= 0)) - 1;
-        seg = __shfl_sync(0xffffffffu, seg, who);
-        at = __shfl_sync(0xffffffffu, seg_before, who);
-        // its pieces again, 32 at a time, in index order
-        const int b = seg / SA_W, bv0 = b * per_block, bv = min(per_block, NV - bv0), pw = (bv + SA_W - 1) / SA_W;
-        const int s0 = min(seg % SA_W * pw, bv), s1 = min(s0 + pw, bv);
-        bool found = false;
-        for (int vb = s0; vb < s1 && !found; vb += 32) {
-          const int v = vb + lane, e0 = (bv0 + v) * PER - skew;
-          unsigned long long w[PER], mm = 0;
-          if (v < s1) {
-            uint4 q;
-            raw *qr = reinterpret_cast<raw *>(&q);
-            if (e0 >= 0 && e0 + PER <= a.V) {
-              q = ld_cg16(x + e0);
-            } else {
-#pragma unroll
-              for (int j = 0; j < PER; ++j) qr[j] = e0 + j >= 0 && e0 + j < a.V ? __ldcg(x + e0 + j) : FILL;
-            }
-#pragma unroll
-            for (int j = 0; j < PER; ++j) {
-              const float f = E::up(qr[j]);
-              const unsigned long long key =
-                  (unsigned long long)key_of<E>(qr[j]) << SA_IDX_BITS | (unsigned)((1 << SA_IDX_BITS) - 1 - (e0 + j));
-              const double wd = weigh.finite(f);
-              w[j] = f == f && key >= last && wd >= mp ? Weigher::fixed(wd) : 0;
-              mm += w[j];
-            }
+        if (seg >= 0) {  // one lane
+          s.bin = seg;
+          s.before = seg_before;
+          s.in_bin = target;
+        }
+      }
+      __syncthreads();
+      // its pieces again, one a thread, in index order
+      const int seg = s.bin;
+      unsigned long long at = s.before;
+      const unsigned long long target = s.in_bin;
+      const int b = seg / SA_W, bv0 = b * per_block, bv = min(per_block, NV - bv0), pw = (bv + SA_W - 1) / SA_W;
+      const int s0 = min(seg % SA_W * pw, bv), s1 = min(s0 + pw, bv);
+      for (int vb = s0; vb < s1 && at <= target; vb += SA_T) {
+        const int v = vb + t, e0 = (bv0 + v) * PER - skew;
+        unsigned long long w[PER], mm = 0;
+        if (v < s1) {
+          uint4 q;
+          raw *qr = reinterpret_cast<raw *>(&q);
+          if (e0 >= 0 && e0 + PER <= a.V) {
+            q = ld_cg16(x + e0);
           } else {
 #pragma unroll
-            for (int j = 0; j < PER; ++j) w[j] = 0;
+            for (int j = 0; j < PER; ++j) qr[j] = e0 + j >= 0 && e0 + j < a.V ? __ldcg(x + e0 + j) : FILL;
           }
-          const unsigned long long ms = warp_scan(mm);
-          unsigned long long run2 = at + ms - mm;
 #pragma unroll
           for (int j = 0; j < PER; ++j) {
-            if (run2 <= target && target < run2 + w[j]) {
-              finish(e0 + j);
-              found = true;
-            }
-            run2 += w[j];
+            const float f = E::up(qr[j]);
+            const unsigned long long key =
+                (unsigned long long)key_of<E>(qr[j]) << SA_IDX_BITS | (unsigned)((1 << SA_IDX_BITS) - 1 - (e0 + j));
+            const double wd = weigh.finite(f);
+            w[j] = f == f && key >= last && wd >= mp ? Weigher::fixed(wd) : 0;
+            mm += w[j];
           }
-          found = __any_sync(0xffffffffu, found);
-          at += __shfl_sync(0xffffffffu, ms, 31);
+        } else {
+#pragma unroll
+          for (int j = 0; j < PER; ++j) w[j] = 0;
         }
+        const unsigned long long ms = warp_scan(mm);
+        unsigned long long before, total;
+        __syncthreads();  // (the slots of the round before have been read)
+        block_offsets(ms, s.scan[1], before, total);
+        unsigned long long run2 = at + before + ms - mm;
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+          if (run2 <= target && target < run2 + w[j]) finish(e0 + j);
+          run2 += w[j];
+        }
+        at += total;
       }
       return;
     }
