@@ -19,7 +19,12 @@
 // the order-preserving integer key inside the chosen bin, until a bin is one key.
 //
 // What bounds it: a pass over the staged row costs about 10 (counts) to 30 (weights in fp64) issue slots an element,
-// against 2 to 4 bytes to load; the cluster's three barriers and the sort are latency, some microseconds a row.
+// against 2 to 4 bytes to load; the cluster's four barriers and the sort are latency, some microseconds a row. Rows of
+// 65536: 256 in fp32 take 117 us with a nucleus alone (0.57 TB/s; two blocks an SM issue 2.2 instructions a clock and the
+// fp64 pipe is 18 % busy), in bf16 62 us unfiltered and 52 us with a top_k of 50 (no fp64 pass over the row); one row in
+// bf16 13 us. The list replaces an exact histogram over the whole row, several passes (16 rows with a top_k of 5000,
+// which still take them: 70 us). The other blocks leave before the list is sorted, so the next row starts on their SMs
+// (124 -> 120 us), and the whole block searches the piece that holds the token (120 -> 117; a warp did it before).
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>

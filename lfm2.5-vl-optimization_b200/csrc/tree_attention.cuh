@@ -67,8 +67,9 @@ struct Request {
   }
 };
 
-// Keys per split of the kernel for odd pages, the same for every request (so that splits of long and short requests take the same time): the
-// longest request cut into S, in whole tiles. For a whole block; `red` is one int of its shared memory.
+// Keys per split of the kernel for pages that are not multiples of 8, the same for every request (so that splits of long
+// and short requests take the same time): the longest request cut into S, in whole tiles. For a whole block; `red` is one
+// int of its shared memory.
 __device__ __forceinline__ int split_chunk(const TreeArgs &a, int *red) {
   if (threadIdx.x == 0) *red = 1;
   __syncthreads();

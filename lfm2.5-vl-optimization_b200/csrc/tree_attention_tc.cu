@@ -13,6 +13,14 @@
 // than 2^8 since the last time (the probabilities then reach at most 2^8, as exact as below 1), rarely after the first
 // tiles.
 //
+// What bounds it, by the rows a KV head has (bf16, 32 heads over 8 KV heads of 64, pages of 64). Few rows: the cache's
+// bytes. 64 requests x 1 token x 8000 positions: 185 us, 5.7 TB/s, 87 % of the measured copy rate; 32 requests x 16
+// drafts x 500 to 4000 positions: 50 us of which 27 are the stream's, the rest begins and ends units (queries in, first
+// tiles, O out, the join). Many rows: the softmax. 16 requests x 64 drafts x 8000 to 32000 positions: 319 us, 2.1 TB/s and
+// 0.37 PFLOP/s; without its exponentials the same loop takes 243 us, without the softmax 201 us. Two row tiles a block
+// halve the reads of the cache there; with one row tile (at most 128 rows a request) two blocks share an SM and one
+// loads while the other is in its softmax.
+//
 // Every wait is bounded (about a second of SM clocks); a wait that gives up sets the device error word that
 // lfm2q_check_device reports, and the block ends without writing its rows.
 #include <cuda.h>
@@ -301,7 +309,7 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
                         g.n0 + g.tok0 + p * tpt);
       }
       // Page numbers come a tile ahead: their load takes as long as a tile (loaded where they were used, the loading warp
-      // bounded the kernel, 217 us where it is 170 now).
+      // bounded the kernel, 217 us where it is 185 now).
       const int *table = a.table + (size_t)g.b * a.width;
       int idx[2], y[2], ahead[2];
 #pragma unroll

@@ -443,8 +443,8 @@ class DecodeGemvExt:
 
     # -------------------------------------------------- batches of requests over a paged cache (include/lfm2q.h)
     # These are called a few times a decode iteration on small work, so the checks are written to cost little on the
-    # host: one helper call a tensor that returns its pointer, messages formed only on failure (16-20 us a call with
-    # the checks above, 8-10 us so).
+    # host: one helper call a tensor that returns its pointer, messages formed only on failure (17-20 us a call with
+    # the checks above, 8-13 us so, of which the launch is 4-7).
     def kv_slots(self, lens, new_lens, table, free, n_free, page, got, cu, positions, slots):
         """Block tables and slot maps from request lengths (no counterpart in the reference; lfm2q_kv_slots has the
         rules). lens, new_lens, got int32 [B], table int32 [B, max_pages], free int32 [num_pages] with n_free int32 [1]
@@ -607,7 +607,8 @@ class GemvChain:
 
 def check_device(clear=False):
     """Raise RuntimeError if a bounded pipeline wait inside a tcgen05 GEMM, the decode attention or the tree attention
-    gave up since the last clear (the outputs of that work are then invalid). Synchronises with the current device. clear: reset the word."""
+    gave up since the last clear (the outputs of that work are then invalid). Synchronises with the current device.
+    clear: reset the word."""
     st = _capi.lib().lfm2q_check_device(int(bool(clear)))
     if st != _capi.OK:
         raise RuntimeError(_capi.lib().lfm2q_last_error().decode() or f"lfm2q_check_device: status {st}")
