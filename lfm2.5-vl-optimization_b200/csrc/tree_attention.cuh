@@ -84,12 +84,13 @@ __device__ __forceinline__ int split_chunk(const TreeArgs &a, int *red) {
 // How the tensor-core kernel deals out work. A unit is one KV head and up to `rows` rows of one request; the tiles of all
 // units, in the order (request, KV head, row tile, position), are one line that is cut into equal stretches of `quota`
 // tiles, one a block: every block has the same work whatever the lengths, and a unit is split only where a stretch ends.
-// Every unit counts TA_UNIT_COST tiles more than it has, for its beginning and end in a block (about 3 us against 1 us a
-// tile: without it blocks with many short units ended last, 52 us where the mean was 38). No unit may fall into more
-// than S stretches: quota >= longest / (S - 1). With S = 1 whole units are dealt out.
-constexpr int TA_UNIT_COST = 3;
+// Every unit counts some tiles more than it has, for its beginning and end in a block: by a fit over blocks of one to four
+// units 3.9 us, a tile 0.56 us at D = 64 with two blocks an SM (32 requests x 16 drafts: 50 us with 3 tiles, 47 with 5 to
+// 9; 100 requests x 4: 89, 80 with 7), twice that at D = 128. No unit may fall into more than S stretches: quota >=
+// longest / (S - 1). With S = 1 whole units are dealt out.
+__host__ __device__ constexpr int unit_cost(int D) { return D == 64 ? 7 : 3; }
 struct TreePlan {
-  int rows;
+  int rows, cost;  // rows of a unit; tiles that it counts beside its own
   long long quota;
   int b;            // request of the block's first tile
   long long base;   // tiles before that request
@@ -98,7 +99,7 @@ struct TreePlan {
   int r_n0, r_T, r_ctx, r_len;  // lane i: request i (of the first 32)
   static __device__ __forceinline__ int tiles(const Request &rq) { return (rq.len + TA_KEYS - 1) / TA_KEYS; }
   // what a unit of n tiles takes of the line
-  static __device__ __forceinline__ int span(const TreeArgs &a, int n) { return a.S == 1 ? 1 : n + TA_UNIT_COST; }
+  __device__ __forceinline__ int span(const TreeArgs &a, int n) const { return a.S == 1 ? 1 : n + cost; }
   __device__ __forceinline__ int units(const TreeArgs &a, const Request &rq) const {
     return a.NKV * ((rq.T * a.G + rows - 1) / rows);
   }
@@ -119,7 +120,8 @@ struct TreePlan {
     return rq;
   }
   // For a whole warp: the stretch of block c of `blocks`.
-  __device__ __forceinline__ TreePlan(const TreeArgs &a, int rows_, int blocks, int c) : rows(rows_), b(a.B), base(0) {
+  __device__ __forceinline__ TreePlan(const TreeArgs &a, int rows_, int cost_, int blocks, int c)
+      : rows(rows_), cost(cost_), b(a.B), base(0) {
     const int lane = threadIdx.x & 31;
     int longest = 1;
     long long total = 0, first = 0;
@@ -144,7 +146,9 @@ struct TreePlan {
     longest = __reduce_max_sync(0xffffffffu, longest);
     quota = total < 0x7fff0000 ? ((int)total + blocks - 1) / blocks : (total + blocks - 1) / blocks;
     if (a.S > 1) quota = max(quota, (long long)((longest + a.S - 2) / (a.S - 1)));
-    quota = max(quota, 1ll);
+    // A part of few tiles and many rows writes, and the joining kernel reads, more than it loads: a tile for every 64 rows
+    // (5 requests x 13 drafts, 104 rows of 128: 21.6 us with a tile a part, 19.3 with two).
+    quota = max(quota, (long long)(min(rows, a.max_q * a.G) + 63) / 64);
     const long long x0 = quota * c;
     count = max(0ll, min(quota, total - x0));
     long long run = 0;

@@ -151,6 +151,15 @@ __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32
       "r"(taddr)
       : "memory");
 }
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {  // and waits
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+      "tcgen05.wait::ld.sync.aligned;"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr)
+      : "memory");
+}
 // wait for this thread's TMEM loads, the registers tied to the wait so that no use of them moves before it
 __device__ __forceinline__ void tmem_ld_wait(uint32_t (&r)[32]) {
   asm volatile("tcgen05.wait::ld.sync.aligned;" : TT_REGS32(r, TT_TIE) : : "memory");
@@ -178,7 +187,8 @@ struct TcShape {
   static constexpr int STAGES = PIPE == 1 ? (D == 64 ? 5 : 2) : (D == 64 ? 8 : 4);
   static constexpr int Q_BYTES = HALVES * TT_ATOM;   // per row tile
   static constexpr int KV_BYTES = HALVES * TT_HALF;  // a K (or V) tile
-  static constexpr int SMEM = PIPE * Q_BYTES + 2 * STAGES * KV_BYTES + 1024;  // room to align the base to 1024
+  static constexpr int OUT_BYTES = 2048;             // per softmax warp: 64 bytes of its 32 rows on their way out
+  static constexpr int SMEM = PIPE * (Q_BYTES + 4 * OUT_BYTES) + 2 * STAGES * KV_BYTES + 1024;  // 1024: to align the base
 };
 
 // A stretch of one unit's tiles. The loading warp works out the block's segments and hands each to the other warps in
@@ -189,10 +199,87 @@ struct Segment {
   int part, parts;            // which part of the unit this is, of how many
 };
 
+// A warp's rows of O times inv, to base + rel D: in the output's type, or fp32. 16 dims at a time go through shared memory
+// (`stage`, 2 KB), so that two or four lanes write one row's bytes: stores of 16 bytes to 32 rows at once take 32 turns of
+// the memory pipe each (5 requests x 13 drafts, 104 rows of 128: 19.3 us so, 18.0 us through shared memory). Out of line:
+// the registers of the loop over the tiles are full.
+template <class T, int D, bool OUT>
+__device__ __noinline__ void rows_out(uint32_t t_o, float inv, uint4 *stage, void *base, int rel, int rows) {
+  constexpr int PIECES = OUT ? 2 : 4, LG = OUT ? 1 : 2, BYTES = D * (OUT ? 2 : 4);  // pieces of 16 bytes a row
+  const int lane = threadIdx.x & 31, x = lane & (PIECES - 1);
+  uint8_t *dst[PIECES];
+  const uint4 *src[PIECES];
+#pragma unroll
+  for (int k = 0; k < PIECES; ++k) {
+    const int r = (32 * k + lane) >> LG;
+    dst[k] = static_cast<uint8_t *>(base) + (size_t)__shfl_sync(0xffffffffu, rel, r) * BYTES + 16 * x;
+    src[k] = stage + (r << LG) + (x ^ (r >> LG & (PIECES - 1)));
+  }
+#pragma unroll 1
+  for (int c = 0; c < D / 16; ++c) {
+    uint32_t o[16];
+    tmem_ld16(t_o + 16 * c, o);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * inv);
+    if (OUT) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) o[j] = Pair<T>::pack(__uint_as_float(o[2 * j]), __uint_as_float(o[2 * j + 1]));
+    }
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k)
+      stage[(lane << LG) + (k ^ (lane >> LG & (PIECES - 1)))] =
+          make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+    __syncwarp();
+    uint4 w[PIECES];
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) w[k] = *src[k];
+    __syncwarp();
+#pragma unroll
+    for (int k = 0; k < PIECES; ++k) {
+      if ((32 * k + lane) >> LG < rows) *reinterpret_cast<uint4 *>(dst[k]) = w[k];
+      dst[k] += 16 * PIECES;
+    }
+  }
+}
+
+// The drafts of `extra`, left out of the second product, added to a row of O: the score again from global memory, and
+// p v. Rare, so out of line. For a whole warp.
+template <class T, int D>
+__device__ __noinline__ void add_apart(const TreeArgs &a, unsigned long long extra, uint32_t t_o, size_t row, int kvh,
+                                       int ctx, const int *table, float m) {
+  const uint32_t *qr = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(a.q) + row * D);
+  for (int c = 0; c < D / 32; ++c) {
+    uint32_t o[32];
+    tmem_ld32(t_o + 32 * c, o);
+    tmem_ld_wait(o);
+    for (unsigned long long rest = extra; rest; rest &= rest - 1) {
+      const int t = ctx + __ffsll(rest) - 1;
+      const size_t at = (((size_t)__ldcg(table + t / a.page) * a.NKV + kvh) * a.page + t % a.page) * D;
+      const uint32_t *kr = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(a.kc) + at);
+      const uint32_t *vr = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(a.vc) + at) + 16 * c;
+      float dot = 0.f;
+      for (int j = 0; j < D / 2; ++j) {
+        const float2 x = Pair<T>::up(__ldcg(qr + j)), y = Pair<T>::up(__ldcg(kr + j));
+        dot += x.x * y.x + x.y * y.y;
+      }
+      const float pr = ex2(fmaf(dot, a.scale_log2, m == -INFINITY ? 0.f : -m));
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float2 v = Pair<T>::up(__ldcg(vr + j));
+        o[2 * j] = __float_as_uint(__uint_as_float(o[2 * j]) + pr * v.x);
+        o[2 * j + 1] = __float_as_uint(__uint_as_float(o[2 * j + 1]) + pr * v.y);
+      }
+    }
+    __syncwarp();
+    tmem_st32(t_o + 32 * c, o);
+  }
+  tmem_st_wait();
+}
+
 template <class T, int D, int PIPE>
 __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
-                   const __grid_constant__ CUtensorMap tmV, const TreeArgs a, int box, int tpt) {
+                   const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TreeArgs a, int box, int tpt) {
   using L = TcShape<D, PIPE>;
   constexpr int STAGES = L::STAGES, HALVES = L::HALVES;
   constexpr bool BF = std::is_same<T, bf16>::value;
@@ -250,7 +337,7 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
 
   if (warp == W_TMA) {
     // ---------------------------------------------------------------- segments, queries, K and V tiles
-    const TreePlan plan(a, PIPE * tpt * a.G, gridDim.x, blockIdx.x);
+    const TreePlan plan(a, PIPE * tpt * a.G, unit_cost(D), gridDim.x, blockIdx.x);
     const int boxes = TA_KEYS / box, page_step = TA_KEYS / a.page, row_step = TA_KEYS % a.page;
     long long left = plan.count, off = plan.off, base = plan.base;
     int b = plan.b, st = 0, ph = 1;  // a fresh barrier passes a wait for the phase before its first
@@ -455,6 +542,8 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
     const int pipe = warp >> 2, quarter = warp & 3, row = threadIdx.x & (TT_ROWS - 1);
     const uint32_t tbase = tmem + 256 * pipe + ((uint32_t)(quarter * 32) << 16);
     const uint32_t t_o = tbase + L::O_COL;
+    const int my_tok = row / a.G, my_head = row - my_tok * a.G;
+    uint4 *out_stage = reinterpret_cast<uint4 *>(smem + PIPE * L::Q_BYTES + 2 * STAGES * L::KV_BYTES + warp * L::OUT_BYTES);
     uint32_t cnt = 0, seg = 0, pairs = 0;  // tiles, segments, segments of two tiles or more
     int st = 0, ph = 0, edges = 0;
     bool ok = true;
@@ -468,7 +557,7 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
       const bool active = quarter * 32 < toks * a.G, has = row < toks * a.G;
       unsigned long long see = 0;
       if (has) {
-        const int tok = tok0 + row / a.G;
+        const int tok = tok0 + my_tok;
         see = a.mask ? __ldcg(a.mask + g->n0 + tok) : (tok >= 63 ? ~0ull : (2ull << tok) - 1);
       }
       float m = -INFINITY, l = 0.f;
@@ -522,11 +611,16 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
             }
             sum = (sum0.x + sum0.y) + (sum1.x + sum1.y);
           };
-          probabilities();
-          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          auto largest = [&]() {
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) mx[j & 3] = max3(mx[j & 3], __uint_as_float(s0[j]), __uint_as_float(s1[j]));
-          const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+            for (int j = 0; j < 32; ++j) mx[j & 3] = max3(mx[j & 3], __uint_as_float(s0[j]), __uint_as_float(s1[j]));
+            return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
+          };
+          // (a unit's first tile starts with its own: 0.4 us of 11.5 for one token; of no use to the long units of PIPE 2)
+          if (PIPE == 1 && n == 0) m = largest();
+          probabilities();
+          const float top = largest();
           const bool grow = top > m + TT_SLACK || (m == -INFINITY && top > -INFINITY);
           if (__any_sync(0xffffffffu, grow)) {
             const float corr = grow ? ex2(m - top) : 1.f;  // 0 while the row has seen nothing
@@ -622,60 +716,19 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
       if (!active) continue;
       tc_fence_after();
       const int parts = g->parts;
-      const size_t out_row = (size_t)(g->n0 + tok0 + row / a.G) * a.NQ + g->kvh * a.G + row % a.G;
-      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int rel = (tok0 + my_tok) * a.NQ + my_head, rows = toks * a.G - quarter * 32;
+      const size_t first_row = (size_t)g->n0 * a.NQ + g->kvh * a.G;
+      const float inv = l == 0.f ? 0.f : __fdividef(1.f, l);
       const unsigned long long extra = *(volatile unsigned long long *)&apart[seg & 3] & see;
-      float *part = ws_acc(a, D, g->part, out_row);
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_ld32(t_o + 32 * c, o);
-        tmem_ld_wait(o);
-        if (extra && has) {  // rare: the score again from global memory, and p v added
-          const uint32_t *qr = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(a.q) + out_row * D);
-          for (unsigned long long rest = extra; rest; rest &= rest - 1) {
-            const int t = ctx + __ffsll(rest) - 1;
-            const size_t at =
-                (((size_t)__ldcg(a.table + (size_t)g->b * a.width + t / a.page) * a.NKV + g->kvh) * a.page + t % a.page) * D;
-            const uint32_t *kr = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(a.kc) + at);
-            const uint32_t *vr = reinterpret_cast<const uint32_t *>(reinterpret_cast<const T *>(a.vc) + at) + 16 * c;
-            float dot = 0.f;
-            for (int j = 0; j < D / 2; ++j) {
-              const float2 x = Pair<T>::up(__ldcg(qr + j)), y = Pair<T>::up(__ldcg(kr + j));
-              dot += x.x * y.x + x.y * y.y;
-            }
-            const float pr = ex2(fmaf(dot, a.scale_log2, m == -INFINITY ? 0.f : -m));
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const float2 v = Pair<T>::up(__ldcg(vr + j));
-              o[2 * j] = __float_as_uint(__uint_as_float(o[2 * j]) + pr * v.x);
-              o[2 * j + 1] = __float_as_uint(__uint_as_float(o[2 * j + 1]) + pr * v.y);
-            }
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * inv);
-        if (has) {
-          if (parts == 1) {
-            uint4 *dst = reinterpret_cast<uint4 *>(reinterpret_cast<T *>(a.out) + out_row * D + 32 * c);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = Pair<T>::pack(__uint_as_float(o[8 * j + 2 * e]), __uint_as_float(o[8 * j + 2 * e + 1]));
-              dst[j] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-          } else {
-            uint4 *dst = reinterpret_cast<uint4 *>(part + 32 * c);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
-          }
-        }
-      }
+      if (__any_sync(0xffffffffu, extra != 0))
+        add_apart<T, D>(a, extra, t_o, first_row + rel, g->kvh, ctx, a.table + (size_t)g->b * a.width, m);
+      if (parts == 1)
+        rows_out<T, D, true>(t_o, inv, out_stage, reinterpret_cast<T *>(a.out) + first_row * D, rel, rows);
+      else
+        rows_out<T, D, false>(t_o, inv, out_stage, ws_acc(a, D, g->part, first_row), rel, rows);
       if (a.S > 1 && has) {
-        float *info = ws_row(a, D, out_row);
-        if (parts > 1) info[1 + g->part] = l == 0.f ? -INFINITY : m + log2f(l);
+        float *info = ws_row(a, D, first_row + rel);
+        if (parts > 1) info[1 + g->part] = l == 0.f ? -INFINITY : m + __log2f(l);
         if (g->part == 0) reinterpret_cast<int *>(info)[0] = parts;
       }
       tc_fence_before();  // O has been read, before the next segment's first product (ordered by its P)
