@@ -411,67 +411,73 @@ __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
     }
 }
 
-// One warp per (query, head): the parts joined in order. A row of one part has been written by its block.
+// D / 4 lanes per (query, head): the parts joined in order. A row of one part has been written by its block. What bounds
+// it is a chain of loads (lengths, the parts' sums, the parts), so the sums come in one go, UNR parts are in flight
+// together and, at D = 64, two rows share a warp (32 requests x 16 drafts in all: 47.4 us with a row a warp, 44.3 so). UNR
+// 16 where there may be many parts, which are few rows (one token: 10.8 us, 11.1 with 8), else 8, which leaves room for
+// more warps (32 x 16 drafts: 44.3 us, 46.6 with 16, 44.3 with 4).
 constexpr int TC_WARPS = 4;
-constexpr int UNR = 8;
-template <class T, int D>
+template <class T, int D, int UNR>
 __global__ void __launch_bounds__(32 * TC_WARPS) tree_combine_kernel(const TreeArgs a) {
-  constexpr int DPL = D / 32;  // dims per lane
+  constexpr int LANES = D / 4, ROWS = 32 / LANES;  // of a row; rows of a warp
   pdl_trigger();
   pdl_wait();
-  const int lane = threadIdx.x & 31, unit = blockIdx.x * TC_WARPS + (threadIdx.x >> 5);
-  const int b = blockIdx.y, i = unit / a.NQ, h = unit % a.NQ;
+  const int lane = threadIdx.x & 31, sub = lane % LANES;
+  const int unit = (blockIdx.x * TC_WARPS + (threadIdx.x >> 5)) * ROWS + lane / LANES;
+  const int b = blockIdx.y, i = unit / a.NQ, h = unit - i * a.NQ;
   const Request rq(a, b);
-  if (i >= rq.T) return;
-  const size_t row = (size_t)(rq.n0 + i) * a.NQ + h;
+  const bool live = i < rq.T;
+  const size_t row = live ? (size_t)(rq.n0 + i) * a.NQ + h : 0;
   const float *info = ws_row(a, D, row);
-  // one load brings the number of parts (lane 0) and up to 31 parts' logarithms (lane 1 + part)
-  const float first = lane <= a.S ? __ldcg(info + lane) : -INFINITY;
+  // two loads at once bring the number of parts (lane 0) and the first parts' logarithms (word 1 + part)
+  const float first = live && sub <= a.S ? __ldcg(info + sub) : -INFINITY;
+  const float second = live && LANES + sub <= a.S ? __ldcg(info + LANES + sub) : -INFINITY;
   // (held to S: after a wait that gave up the words were never written)
-  const int parts = min(__shfl_sync(0xffffffffu, __float_as_int(first), 0), a.S);
-  if (parts <= 1) return;
-  float M = lane > 0 && lane <= parts ? first : -INFINITY;
-  for (int s = 31 + lane; s < parts; s += 32) M = fmaxf(M, __ldcg(info + 1 + s));
-  M = warp_max(M);
+  int parts = min(__shfl_sync(0xffffffffu, __float_as_int(first), 0, LANES), a.S);
+  if (!live || parts <= 1) parts = 0;
+  const int most = __reduce_max_sync(0xffffffffu, parts);
+  if (most == 0) return;
+  float M = sub > 0 && sub <= parts ? first : -INFINITY;
+  if (LANES + sub <= parts) M = fmaxf(M, second);
+  for (int s = 2 * LANES - 1 + sub; s < parts; s += LANES) M = fmaxf(M, __ldcg(info + 1 + s));
+#pragma unroll
+  for (int o = LANES / 2; o > 0; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
   const float ms = M == -INFINITY ? 0.f : M;
-  float L = 0.f, acc[DPL];
+  float L = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s0 = 0; s0 < most; s0 += UNR) {  // UNR parts in flight
+    float4 v[UNR];
 #pragma unroll
-  for (int j = 0; j < DPL; ++j) acc[j] = 0.f;
-  for (int s0 = 0; s0 < parts; s0 += UNR) {  // UNR parts in flight
-    float2 v[UNR][DPL / 2];
-#pragma unroll
-    for (int u = 0; u < UNR; ++u) {
-      const float *p = ws_acc(a, D, min(s0 + u, parts - 1), row) + DPL * lane;
-#pragma unroll
-      for (int j = 0; j < DPL; j += 2) v[u][j / 2] = __ldcg(reinterpret_cast<const float2 *>(p + j));
-    }
+    for (int u = 0; u < UNR; ++u)
+      v[u] = s0 + u < parts ? __ldcg(reinterpret_cast<const float4 *>(ws_acc(a, D, s0 + u, row) + 4 * sub))
+                            : make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int u = 0; u < UNR; ++u) {
       const int s = s0 + u;
-      const float lse = s < 31 ? __shfl_sync(0xffffffffu, first, (s + 1) & 31) : s < parts ? __ldcg(info + 1 + s) : 0.f;
-      if (s < parts) {
-        const float c = ex2(lse - ms);
-        L += c;
-#pragma unroll
-        for (int j = 0; j < DPL; j += 2) {
-          acc[j] += v[u][j / 2].x * c;
-          acc[j + 1] += v[u][j / 2].y * c;
-        }
-      }
+      float lse = __shfl_sync(0xffffffffu, s + 1 < LANES ? first : second, (s + 1) & (LANES - 1), LANES);
+      if (s + 1 >= 2 * LANES && s < parts) lse = __ldcg(info + 1 + s);
+      const float c = s < parts ? ex2(lse - ms) : 0.f;
+      L += c;
+      acc.x += v[u].x * c;
+      acc.y += v[u].y * c;
+      acc.z += v[u].z * c;
+      acc.w += v[u].w * c;
     }
   }
+  if (parts == 0) return;
   const float inv = L == 0.f ? 0.f : 1.f / L;
-  uint32_t *dst = reinterpret_cast<uint32_t *>(reinterpret_cast<T *>(a.out) + row * D + DPL * lane);
-#pragma unroll
-  for (int j = 0; j < DPL; j += 2) dst[j / 2] = Pair<T>::pack(acc[j] * inv, acc[j + 1] * inv);
+  *reinterpret_cast<uint2 *>(reinterpret_cast<T *>(a.out) + row * D + 4 * sub) =
+      make_uint2(Pair<T>::pack(acc.x * inv, acc.y * inv), Pair<T>::pack(acc.z * inv, acc.w * inv));
 }
 
 template <class T, int D>
 cudaError_t launch_combine(const TreeArgs &a, bool pdl, cudaStream_t st) {
+  auto kernel = a.S <= 8 ? tree_combine_kernel<T, D, 8> : tree_combine_kernel<T, D, 16>;
+  constexpr int ROWS = TC_WARPS * 128 / D;  // of a block
   cudaLaunchAttribute attr;
   const cudaLaunchConfig_t cfg =
-      pdl_config(dim3((a.max_q * a.NQ + TC_WARPS - 1) / TC_WARPS, a.B), dim3(32 * TC_WARPS), pdl, st, &attr);
-  return cudaLaunchKernelEx(&cfg, tree_combine_kernel<T, D>, a);
+      pdl_config(dim3((a.max_q * a.NQ + ROWS - 1) / ROWS, a.B), dim3(32 * TC_WARPS), pdl, st, &attr);
+  return cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 template <class T, int D, int WM, int WK, int MT, int STAGES>
