@@ -270,7 +270,8 @@ int lfm2q_qk_norm_rope_kv_paged(const uint16_t *qkv, int64_t row_stride, const u
  * sees every position < ctx[b], and ctx[b] + j where bit j of mask[cu[b] + i] is set (mask NULL: j <= i). out [N, NQ, D]
  * = softmax(scale q.k) v; a query that sees nothing gives zeros. Rows outside the requests, and those past max_q of a
  * request, are left as they were. NQ = G NKV, G <= 64; D 64 or 128; scale > 0. A position whose page is outside
- * [0, num_pages), or past the table, is not seen.
+ * [0, num_pages), or past the table, is not seen. B * NKV * (tiles of 128 rows, of whole queries, that max_q queries take)
+ * * (max_pages * page / 64 + 8) must be below 2^31 - 2^16.
  * The positions of a request are cut into at most S parts (lfm2q_tree_attention_splits suggests a number): with S > 1 ws,
  * fp32, N * NQ * S * (D + 2) words, holds the parts' results until a second kernel joins them (no value needs to be set
  * before; calls that may run at the same time need their own); S = 1 needs none. Results do not depend on what ws held;

@@ -482,6 +482,10 @@ int lfm2q_tree_attention(const uint16_t *q, const uint16_t *kc, const uint16_t *
   REQUIRE((long long)max_pages * page <= (1ll << 30), "max_pages * page must be <= 2^30");
   REQUIRE(B <= 65535 && (long long)B * NKV * max_q <= 0x7fffffffLL, "B must be <= 65535 and B * NKV * max_q < 2^31");
   REQUIRE((long long)num_pages * NKV <= 0x7fffffffLL, "num_pages * NKV must be < 2^31");
+  // (a request's rows in tiles of 128, its positions in tiles of 64 and 8 for a beginning and an end)
+  const long long row_tiles = (max_q * (NQ / NKV) + 127) / (128 / (NQ / NKV) * (NQ / NKV));
+  REQUIRE((double)B * NKV * row_tiles * ((double)max_pages * page / 64 + 8) < 2147483648.0 - 65536,
+          "B * NKV * (tiles of 128 rows a request) * (max_pages * page / 64) must be < 2^31");
   REQUIRE(S >= 1 && S <= 65535, "ws [N, NQ, S, D + 2]: need 1 <= S <= 65535");
   REQUIRE(scale > 0.f && scale < 1e30f, "scale must be positive and finite");
   if (N == 0 || B == 0) return LFM2Q_OK;

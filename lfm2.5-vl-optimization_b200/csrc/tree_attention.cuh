@@ -89,25 +89,26 @@ __device__ __forceinline__ int split_chunk(const TreeArgs &a, int *red) {
 // 9; 100 requests x 4: 89, 80 with 7), twice that at D = 128. No unit may fall into more than S stretches: quota >=
 // longest / (S - 1). With S = 1 whole units are dealt out.
 __host__ __device__ constexpr int unit_cost(int D) { return D == 64 ? 7 : 3; }
+// (The entry point holds the line below 2^31 tiles. Every division here is on the way to the block's first load.)
 struct TreePlan {
   int rows, cost;  // rows of a unit; tiles that it counts beside its own
-  long long quota;
-  int b;            // request of the block's first tile
-  long long base;   // tiles before that request
-  long long off;    // of the block's first tile within it
-  long long count;  // tiles of the block
+  int quota;
+  int x0, count;   // the block's stretch of the line
+  int b;           // request of its first tile
+  int base;        // tiles before that request
   int r_n0, r_T, r_ctx, r_len;  // lane i: request i (of the first 32)
   static __device__ __forceinline__ int tiles(const Request &rq) { return (rq.len + TA_KEYS - 1) / TA_KEYS; }
   // what a unit of n tiles takes of the line
   __device__ __forceinline__ int span(const TreeArgs &a, int n) const { return a.S == 1 ? 1 : n + cost; }
-  __device__ __forceinline__ int units(const TreeArgs &a, const Request &rq) const {
-    return a.NKV * ((rq.T * a.G + rows - 1) / rows);
+  // units of a KV head
+  __device__ __forceinline__ int per_head(const TreeArgs &a, const Request &rq) const {
+    return rq.T * a.G <= rows ? 1 : (rq.T * a.G + rows - 1) / rows;
   }
-  __device__ __forceinline__ long long weight(const TreeArgs &a, const Request &rq, int &n) const {
+  __device__ __forceinline__ int weight(const TreeArgs &a, const Request &rq, int &n) const {
     n = 0;
     if (rq.T == 0) return 0;
     n = tiles(rq);
-    return (long long)units(a, rq) * span(a, n);
+    return a.NKV * per_head(a, rq) * span(a, n);
   }
   // request i, for a whole warp: of the first 32 without another load
   __device__ __forceinline__ Request request(const TreeArgs &a, int i) const {
@@ -121,16 +122,15 @@ struct TreePlan {
   }
   // For a whole warp: the stretch of block c of `blocks`.
   __device__ __forceinline__ TreePlan(const TreeArgs &a, int rows_, int cost_, int blocks, int c)
-      : rows(rows_), cost(cost_), b(a.B), base(0) {
+      : rows(rows_), cost(cost_), x0(0), count(0), b(a.B), base(0) {
     const int lane = threadIdx.x & 31;
-    int longest = 1;
-    long long total = 0, first = 0;
+    int longest = 1, total = 0, first = 0;
     r_n0 = r_T = r_ctx = r_len = 0;
 #pragma unroll 4
     for (int i = lane; i < a.B; i += 32) {
       int n;
       const Request rq(a, i);
-      const long long w = weight(a, rq, n);
+      const int w = weight(a, rq, n);
       if (i == lane) {
         first = w;
         r_n0 = rq.n0;
@@ -141,36 +141,36 @@ struct TreePlan {
       total += w;
       longest = max(longest, n);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+    total = (int)__reduce_add_sync(0xffffffffu, (unsigned)total);
     longest = __reduce_max_sync(0xffffffffu, longest);
-    quota = total < 0x7fff0000 ? ((int)total + blocks - 1) / blocks : (total + blocks - 1) / blocks;
-    if (a.S > 1) quota = max(quota, (long long)((longest + a.S - 2) / (a.S - 1)));
+    quota = (total + blocks - 1) / blocks;
+    if (a.S > 1 && (long long)quota * (a.S - 1) < longest) quota = (longest + a.S - 2) / (a.S - 1);
     // A part of few tiles and many rows writes, and the joining kernel reads, more than it loads: a tile for every 64 rows
     // (5 requests x 13 drafts, 104 rows of 128: 21.6 us with a tile a part, 19.3 with two).
-    quota = max(quota, (long long)(min(rows, a.max_q * a.G) + 63) / 64);
-    const long long x0 = quota * c;
-    count = max(0ll, min(quota, total - x0));
-    long long run = 0;
-    for (int b0 = 0; count > 0 && b0 < a.B; b0 += 32) {
+    quota = max(quota, (min(rows, a.max_q * a.G) + 63) / 64);
+    if ((long long)quota * c >= total) return;
+    x0 = quota * c;
+    count = min(quota, total - x0);
+    int run = 0;
+    for (int b0 = 0; b0 < a.B; b0 += 32) {
       int n;
-      const long long w = b0 == 0 ? first : b0 + lane < a.B ? weight(a, Request(a, b0 + lane), n) : 0;
-      long long s = w;
+      const int w = b0 == 0 ? first : b0 + lane < a.B ? weight(a, Request(a, b0 + lane), n) : 0;
+      int s = w;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const long long s2 = __shfl_up_sync(0xffffffffu, s, o);
+        const int s2 = __shfl_up_sync(0xffffffffu, s, o);
         if (lane >= o) s += s2;
       }
-      const uint32_t here = __ballot_sync(0xffffffffu, run + s - w <= x0 && x0 < run + s);
+      s += run;
+      const uint32_t here = __ballot_sync(0xffffffffu, s - w <= x0 && x0 < s);
       if (here) {  // one lane
         const int at = __ffs(here) - 1;
         b = b0 + at;
-        base = run + __shfl_sync(0xffffffffu, s - w, at);
+        base = __shfl_sync(0xffffffffu, s - w, at);
         break;
       }
-      run += __shfl_sync(0xffffffffu, s, 31);
+      run = __shfl_sync(0xffffffffu, s, 31);
     }
-    off = x0 - base;
   }
 };
 

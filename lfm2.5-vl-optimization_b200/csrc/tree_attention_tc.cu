@@ -339,8 +339,11 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
     // ---------------------------------------------------------------- segments, queries, K and V tiles
     const TreePlan plan(a, PIPE * tpt * a.G, unit_cost(D), gridDim.x, blockIdx.x);
     const int boxes = TA_KEYS / box, page_step = TA_KEYS / a.page, row_step = TA_KEYS % a.page;
-    long long left = plan.count, off = plan.off, base = plan.base;
-    int b = plan.b, st = 0, ph = 1;  // a fresh barrier passes a wait for the phase before its first
+    int left = plan.count, b = plan.b, base = plan.base, st = 0, ph = 1;  // a fresh barrier passes a wait for phase 1
+    // of request b: tiles of a unit, its span on the line, units of a head and in all; the next unit, tile within it
+    Request rq;
+    int tiles = 0, span = 0, per_head = 1, units = 0, unit = 0, j0 = 0;
+    bool next = true, begun = false;
     uint32_t issued = 0, seg = 0;
     bool ok = true, more = true;
     for (; ok && more; ++seg) {
@@ -348,90 +351,80 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
       Segment g = {};
       int t1 = 0;
       while (left > 0 && b < a.B) {
-        const Request rq = plan.request(a, b);
-        const int units = plan.units(a, rq), n = plan.tiles(rq), span = plan.span(a, n);
-        const long long w = (long long)units * span;
-        if (off >= w) {
-          base += w;
-          off = 0;
+        if (next) {
+          rq = plan.request(a, b);
+          tiles = plan.tiles(rq);
+          span = plan.span(a, tiles);
+          per_head = plan.per_head(a, rq);
+          units = rq.T > 0 ? a.NKV * per_head : 0;
+          unit = begun ? 0 : (plan.x0 - base) / span;
+          j0 = begun ? 0 : plan.x0 - base - unit * span;
+          next = false;
+          begun = true;
+        }
+        if (unit == units) {
+          base += units * span;
           ++b;
+          next = true;
           continue;
         }
-        // (the line fits 32 bits but for batches of some 10^9 tiles, whose divisions are slow)
-        const int unit = (int)(off < 0x7fffffff ? (int)off / span : off / span);
-        const int j0 = (int)(off - (long long)unit * span);
-        const int step = (int)min((long long)(span - j0), left), per_head = units / a.NKV;
-        off += step;
+        const int step = min(span - j0, left), from = j0, u = unit, first = base + unit * span;
         left -= step;
-        const int take = a.S == 1 ? n : min(n - j0, step);
-        if (take <= 0) continue;  // the end of a unit's span holds no tiles
-        long long part = 0, last = 0;
-        if (a.S > 1) {
-          const long long first = base + off - step - j0, q = plan.quota;  // the unit's first tile in the line
-          if (first + n < 0x7fffffff && q < 0x7fffffff) {
-            const int f = (int)first / (int)q;
-            part = ((int)first + j0) / (int)q - f;
-            last = ((int)first + n - 1) / (int)q - f;
-          } else {
-            part = (first + j0) / q - first / q;
-            last = (first + n - 1) / q - first / q;
-          }
+        j0 += step;
+        if (j0 == span) {
+          ++unit;
+          j0 = 0;
         }
-        g = {b, unit / per_head, unit % per_head * PIPE * tpt, rq.n0, rq.T, rq.ctx, j0 * TA_KEYS, take, (int)part,
-             (int)last + 1};
-        t1 = min(rq.len, (j0 + take) * TA_KEYS);
+        const int take = a.S == 1 ? tiles : min(tiles - from, step);
+        if (take <= 0) continue;  // the end of a unit's span holds no tiles
+        // the stretches that hold the unit's first tile and its last, of which this is number blockIdx.x
+        int part0 = blockIdx.x, part1 = part0;
+        if (a.S > 1) {
+          const int end = first + tiles - 1;
+          if (first < plan.x0) part0 = first / plan.quota;
+          if (end - plan.x0 >= plan.quota) part1 = end / plan.quota;
+        }
+        const int kvh = per_head == 1 ? u : u / per_head;
+        g = {b, kvh, (u - kvh * per_head) * PIPE * tpt, rq.n0, rq.T, rq.ctx, from * TA_KEYS, take,
+             (int)blockIdx.x - part0, part1 - part0 + 1};
+        t1 = min(rq.len, (from + take) * TA_KEYS);
         more = true;
         break;
       }
+      // Page numbers come a tile ahead, one lane a box: their load takes as long as a tile (loaded where they were used,
+      // the loading warp bounded the kernel, 217 us where it is 185 now).
+      const int *table = a.table + (size_t)g.b * a.width;
+      const int at0 = g.t0 + lane * box;
+      int idx = at0 / a.page, y = at0 - idx * a.page;
+      int ahead = lane < boxes && at0 < t1 ? __ldcg(table + idx) : -1;
       // the queries' place is free when the last scores of the segment before are done
       ok = warp_wait(smem_addr(&q_empty), (seg & 1) ^ 1, &stop);
       if (!ok) break;
       if (lane == 0) {
         segs[seg & 3] = g;
-        const int tiles_q = more ? min(PIPE, (g.T - g.tok0 + tpt - 1) / tpt) : 0;
+        const int tiles_q = !more ? 0 : PIPE > 1 && g.T - g.tok0 > tpt ? 2 : 1;
         mbar_expect_tx(smem_addr(&q_full), tiles_q * HALVES * tpt * a.G * 128);
         for (int p = 0; p < tiles_q; ++p)
           for (int h = 0; h < HALVES; ++h)
             tma_load_3d(sq + p * L::Q_BYTES + h * TT_ATOM, &tmQ, smem_addr(&q_full), 64 * h, g.kvh * a.G,
                         g.n0 + g.tok0 + p * tpt);
       }
-      // Page numbers come a tile ahead: their load takes as long as a tile (loaded where they were used, the loading warp
-      // bounded the kernel, 217 us where it is 185 now).
-      const int *table = a.table + (size_t)g.b * a.width;
-      int idx[2], y[2], ahead[2];
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int i = lane + 32 * u, t = g.t0 + i * box;
-        idx[u] = t / a.page;
-        y[u] = t - idx[u] * a.page;
-        ahead[u] = i < boxes && t < t1 ? __ldcg(table + idx[u]) : -1;
-      }
       for (int n = 0; n < g.tiles; ++n, ++issued) {
-        const int tile_at = g.t0 + n * TA_KEYS;
-        int pg[2], row[2];
-        uint32_t mine = 0;
-        unsigned long long keys = 0;  // of this lane's boxes
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int i = lane + 32 * u, t = tile_at + i * box;
-          pg[u] = ahead[u];
-          row[u] = y[u];
-          idx[u] += page_step;
-          y[u] += row_step;
-          if (y[u] >= a.page) {
-            y[u] -= a.page;
-            ++idx[u];
-          }
-          ahead[u] = n + 1 < g.tiles && i < boxes && t + TA_KEYS < t1 ? __ldcg(table + idx[u]) : -1;
-          if (pg[u] < 0 || pg[u] >= a.num_pages) {
-            pg[u] = -1;
-          } else {
-            ++mine;
-            const int n_live = min(box, t1 - t);
-            keys |= (n_live >= 64 ? ~0ull : (1ull << n_live) - 1) << (i * box);
-          }
+        const int t = at0 + n * TA_KEYS, pg = ahead, row = y;
+        idx += page_step;
+        y += row_step;
+        if (y >= a.page) {
+          y -= a.page;
+          ++idx;
         }
-        const uint32_t loads = __reduce_add_sync(0xffffffffu, mine);
+        ahead = n + 1 < g.tiles && lane < boxes && t + TA_KEYS < t1 ? __ldcg(table + idx) : -1;
+        const bool there = pg >= 0 && pg < a.num_pages;
+        unsigned long long keys = 0;  // of this lane's box
+        if (there) {
+          const int n_live = min(box, t1 - t);
+          keys = (n_live >= 64 ? ~0ull : (1ull << n_live) - 1) << (lane * box);
+        }
+        const uint32_t loads = __popc(__ballot_sync(0xffffffffu, there));
         const uint32_t klo = __reduce_or_sync(0xffffffffu, (uint32_t)keys),
                        khi = __reduce_or_sync(0xffffffffu, (uint32_t)(keys >> 32));
         ok = warp_wait(smem_addr(&empty[st]), (uint32_t)ph, &stop);
@@ -442,20 +435,14 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
           mbar_expect_tx(bar, 2 * loads * box * 128 * HALVES);
         }
         __syncwarp();
+        if (there) {
+          const uint32_t to = st * L::KV_BYTES + lane * box * 128;
+          const int z = pg * a.NKV + g.kvh;
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (pg[u] >= 0)
+          for (int h = 0; h < HALVES; ++h) tma_load_3d(sk + to + h * TT_HALF, &tmK, bar, 64 * h, row, z);
 #pragma unroll
-            for (int h = 0; h < HALVES; ++h)
-              tma_load_3d(sk + st * L::KV_BYTES + h * TT_HALF + (lane + 32 * u) * box * 128, &tmK, bar, 64 * h, row[u],
-                          pg[u] * a.NKV + g.kvh);
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (pg[u] >= 0)
-#pragma unroll
-            for (int h = 0; h < HALVES; ++h)
-              tma_load_3d(sv + st * L::KV_BYTES + h * TT_HALF + (lane + 32 * u) * box * 128, &tmV, bar, 64 * h, row[u],
-                          pg[u] * a.NKV + g.kvh);
+          for (int h = 0; h < HALVES; ++h) tma_load_3d(sv + to + h * TT_HALF, &tmV, bar, 64 * h, row, z);
+        }
         if (++st == STAGES) {
           st = 0;
           ph ^= 1;
