@@ -62,8 +62,9 @@ def test_tree_attention_refuses_more_tiles_than_its_line_holds():
     """B * NKV * ceil(max_q G / (whole queries of 128 rows)) * (max_pages * page / 64 + 8) < 2^31 - 2^16"""
     ok = [F] * 9 + [_capi.BF16, 20, 1024, 32, 32, 64, 10, 64, 65000, 2, 1, 0.125, None]
     refused("lfm2q_tree_attention", swap(ok, _17=65536), "2^31")  # 1024 * 32 * (65536 + 8)
-    refused("lfm2q_tree_attention", swap(ok, _11=512, _12=32 * 64, _19=3), "2^31")  # two tiles of two queries a request
-    for at in (dict(), dict(_11=512, _12=32 * 64, _19=2), dict(_11=512, _12=32 * 64, _19=1)):
+    # two queries a tile: five take three, 512 * 32 * 3 * 65008 (three take two, 2^31 - 17301504)
+    refused("lfm2q_tree_attention", swap(ok, _11=512, _12=32 * 64, _19=5), "2^31")
+    for at in (dict(), dict(_11=512, _12=32 * 64, _19=3), dict(_11=512, _12=32 * 64, _19=1)):
         st = _capi.lib().lfm2q_tree_attention(*swap(ok, **dict(at, _10=0)))  # N = 0: checked, nothing to do
         assert st == _capi.OK, _capi.lib().lfm2q_last_error()
 
