@@ -21,8 +21,8 @@
 // What bounds it: a pass over the staged row costs about 10 (counts) to 30 (weights in fp64) issue slots an element,
 // against 2 to 4 bytes to load; the cluster's four barriers and the sort are latency, some microseconds a row. Rows of
 // 65536: 256 in fp32 take 117 us with a nucleus alone (0.57 TB/s; two blocks an SM issue 2.2 instructions a clock and the
-// fp64 pipe is 18 % busy), in bf16 62 us unfiltered and 52 us with a top_k of 50 (no fp64 pass over the row); one row in
-// bf16 13 us. The list replaces an exact histogram over the whole row, several passes (16 rows with a top_k of 5000,
+// fp64 pipe is 18 % busy), in bf16 62 us unfiltered and 43 us with a top_k of 50 (no fp64 pass over the row); one row in
+// bf16 10.5 us. The list replaces an exact histogram over the whole row, several passes (16 rows with a top_k of 5000,
 // which still take them: 70 us). The other blocks leave before the list is sorted, so the next row starts on their SMs
 // (124 -> 120 us), and the whole block searches the piece that holds the token (120 -> 117; a warp did it before).
 #include <cooperative_groups.h>
@@ -48,6 +48,7 @@ constexpr int SA_MAX_C = 8;             // blocks per cluster (the portable limi
 constexpr int SA_STAGE = 65 * 1024;     // bytes of a row that one block stages (so that two blocks share an SM) ...
 constexpr int SA_MAX_STAGE = 160 * 1024;  // ... and at most
 constexpr int SA_LIST = 2048;           // elements around the cut
+constexpr int SA_FEW = 128;             // a list (with top_k) that is compared pair by pair
 constexpr int SA_IDX_BITS = 18;
 
 // Element types: raw storage, an order-preserving key (equal keys <=> equal values: -0 takes +0's) and its inverse.
@@ -292,6 +293,71 @@ __device__ __forceinline__ unsigned long long target_of(float u, unsigned long l
 __device__ __forceinline__ unsigned long long mass_needed(float p, unsigned long long total) {
   const double want = ceil(fmax(0.0, (double)p) * (double)total);
   return want < 1.0 ? 1ull : min((unsigned long long)want, total);
+}
+
+// The list of a row with a top_k, n <= SA_FEW: all that is kept is in it, so the token is too. Every element is compared
+// with every other, by as many threads as there are for one, which gives its place in the order of keys and in that of
+// indexes; one warp then sums in both orders. In place of the sort, sums over the block and a second look at the row, each
+// of them barriers and chains (one row with a top_k of 50: 13.3 -> 10.5 us, 64 with 100: 23.2 -> 20.0, 256 with 50: 51.9 -> 42.6).
+template <class E, class F>
+__device__ __forceinline__ void draw_few(SampleShared &s, int n, const Weigher &weigh, double mp, bool use_p,
+                                         const Params &par, F finish) {
+  constexpr unsigned INDEX = (1 << SA_IDX_BITS) - 1, HIGH = 1u << 31;
+  constexpr int EACH = SA_FEW / 32;
+  const int t = threadIdx.x, lane = t & 31, lg = min(5, 31 - __clz(SA_T / n)), many = 1 << lg;  // threads an element
+  const int i = t >> lg, sub = t & (many - 1);
+  const unsigned long long key = i < n ? s.f.key[i] : 0;
+  const unsigned low = (unsigned)key & INDEX;
+  int rank = 0, place = 0;
+#pragma unroll 4
+  for (int j = sub; j < n; j += many) {
+    const unsigned long long k = s.f.key[j];
+    rank += k > key;
+    place += ((unsigned)k & INDEX) > low;  // (the low bits fall as the index rises)
+  }
+  for (int o = 1; o < many; o <<= 1) {
+    rank += __shfl_xor_sync(0xffffffffu, rank, o);
+    place += __shfl_xor_sync(0xffffffffu, place, o);
+  }
+  if (i < n && sub == 0) {
+    const double w = weigh(value_of<E>((uint32_t)(key >> SA_IDX_BITS)));
+    s.f.pre[rank] = rank < par.top_k ? Weigher::fixed(w) : 0;
+    s.f.cum[rank] = place | (w >= mp ? HIGH : 0u);
+    s.f.cnt[place] = INDEX - low;
+  }
+  __syncthreads();
+  if (t >= 32) return;
+  unsigned long long w[EACH], run = 0;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    w[j] = EACH * lane + j < n ? s.f.pre[EACH * lane + j] : 0;
+    run += w[j];
+  }
+  unsigned long long sum = warp_scan(run);
+  run = sum - run;
+  const unsigned long long need = use_p ? mass_needed(par.top_p, __shfl_sync(0xffffffffu, sum, 31)) : ~0ull;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j)
+    if (EACH * lane + j < n) {
+      const uint32_t at = s.f.cum[EACH * lane + j];
+      s.f.key[at & ~HIGH] = run < need && at & HIGH ? w[j] : 0;
+      run += w[j];
+    }
+  __syncwarp();
+  run = 0;
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    w[j] = EACH * lane + j < n ? s.f.key[EACH * lane + j] : 0;
+    run += w[j];
+  }
+  sum = warp_scan(run);
+  run = sum - run;
+  const unsigned long long target = target_of(par.u, __shfl_sync(0xffffffffu, sum, 31));
+#pragma unroll
+  for (int j = 0; j < EACH; ++j) {
+    if (run <= target && target < run + w[j]) finish((int)s.f.cnt[EACH * lane + j]);
+    run += w[j];
+  }
 }
 
 // The row by exact histograms: for any number of ties and any top_k. All blocks of the cluster; the token comes out of
@@ -931,6 +997,10 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
     again = s.again != 0;
     if (!again) {
       if (rank != 0) return;
+      if (use_k && n <= SA_FEW) {
+        draw_few<E>(s, n, weigh, mp, use_p, par, finish);
+        return;
+      }
       // ------------------------------------------------------------ sort the list, find the cut, draw
       int N2 = 64;
       while (N2 < n) N2 *= 2;
