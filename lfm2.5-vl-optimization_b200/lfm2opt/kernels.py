@@ -41,11 +41,11 @@ _FLOAT = {**_HALF, torch.float32: _capi.FP32}
 
 def _arg(t, dtype, name, dev):
     """The device pointer of t, checked: a dense tensor of dtype on device dev."""
+    if t.get_device() == dev != -1 and t.dtype is dtype and t.is_contiguous():  # (-1: not on a GPU)
+        return t.data_ptr()
     if not (t.is_cuda and t.dtype is dtype and t.is_contiguous()):
         raise RuntimeError(f"{name} must be contiguous CUDA, dtype {dtype}")
-    if t.get_device() != dev:
-        raise RuntimeError(f"{name}: every tensor must be on one device")
-    return t.data_ptr()
+    raise RuntimeError(f"{name}: every tensor must be on one device")
 
 
 def _launch(fn, dev, *args):
