@@ -12,8 +12,8 @@
 //
 // Two kernels: tree_attention_tc.cu has the one for pages that are multiples of 8 positions (a TMA box of rows never
 // crosses a page, and eight rows are the swizzle's period); this file the one for other pages, and the join of both.
-// 32 requests x 16 drafts x 500 to 4000 positions, 32 heads over 8 KV heads of 64: 113 us here with pages of 20 or 36,
-// 50 us there with pages of 16 or 64, 54 us with pages of 8.
+// 32 requests x 16 drafts x 500 to 4000 positions, 32 heads over 8 KV heads of 64: 111 us here with pages of 20 or 36,
+// 44 us there with pages of 16 or 64, 49 us with pages of 8.
 //
 // Here a block takes a tile of 64 keys at a time through a ring of cp.async stages, 16 bytes a lane, each with its own
 // page (rows swizzled in 16-byte units, so ldmatrix reads are conflict-free), mma.sync m16n8k16 for both products. What
@@ -512,11 +512,12 @@ cudaError_t launch_rows(const TreeArgs &a, int B, bool pdl, cudaStream_t st) {
 }  // namespace
 
 int tree_attention_splits(int B, int NQ, int NKV, int D, int max_q, long long max_len) {
-  // As many parts as equal stretches (two blocks an SM) cut a unit into, were all requests half as long as the longest;
-  // no more than a part a tile.
-  const long long per_tile = std::max(1, 128 / (NQ / NKV)), units = (long long)B * NKV * ((max_q + per_tile - 1) / per_tile);
-  const long long parts = 2 + (4LL * device_sm_count() + units - 1) / units, tiles = (max_len + TA_KEYS - 1) / TA_KEYS;
-  (void)D;
+  // As many parts as the equal stretches of the blocks cut a unit into, were all requests half as long as the longest; no
+  // more than a part a tile.
+  const int per_tile = std::max(1, 128 / (NQ / NKV)), tiles_q = max_q <= per_tile ? 1 : 2;  // of a unit
+  const long long blocks = (tiles_q == 1 && D == 64 ? 2LL : 1LL) * device_sm_count();
+  const long long units = (long long)B * NKV * ((max_q + tiles_q * per_tile - 1) / (tiles_q * per_tile));
+  const long long parts = 2 + (2 * blocks + units - 1) / units, tiles = (max_len + TA_KEYS - 1) / TA_KEYS;
   return tiles <= 1 ? 1 : (int)std::min(std::min(parts, tiles + 1), 64LL);
 }
 

@@ -84,14 +84,15 @@ __device__ __forceinline__ int split_chunk(const TreeArgs &a, int *red) {
 // How the tensor-core kernel deals out work. A unit is one KV head and up to `rows` rows of one request; the tiles of all
 // units, in the order (request, KV head, row tile, position), are one line that is cut into equal stretches of `quota`
 // tiles, one a block: every block has the same work whatever the lengths, and a unit is split only where a stretch ends.
-// Every unit counts some tiles more than it has, for its beginning and end in a block: by a fit over blocks of one to four
-// units 3.9 us, a tile 0.56 us at D = 64 with two blocks an SM (32 requests x 16 drafts: 50 us with 3 tiles, 47 with 5 to
-// 9; 100 requests x 4: 89, 80 with 7), twice that at D = 128. No unit may fall into more than S stretches: quota >=
-// longest / (S - 1). With S = 1 whole units are dealt out.
-__host__ __device__ constexpr int unit_cost(int D) { return D == 64 ? 7 : 3; }
-// (The entry point holds the line below 2^31 tiles. Every division here is on the way to the block's first load.)
+// Every unit counts TA_UNIT_COST tiles more than it has, for its beginning and end in a block: by a fit over blocks of one
+// to four units 3.9 us, where a tile takes 0.6 us (32 requests x 16 drafts: 50 us with 3 tiles, 47 with 5 to 9; 100
+// requests x 4: 89 and 80; heads of 128, 32 x 16: 92 us with 3, 82 with 5 and 8). No unit may fall into more than S
+// stretches: quota >= longest / (S - 1). With S = 1 whole units are dealt out. The entry point holds the line below 2^31
+// tiles. Every division here is on the way to the block's first load (with 64 bits and three more of them: one token
+// 10.8 us, 10.2 so).
+constexpr int TA_UNIT_COST = 5;
 struct TreePlan {
-  int rows, cost;  // rows of a unit; tiles that it counts beside its own
+  int rows;        // of a unit
   int quota;
   int x0, count;   // the block's stretch of the line
   int b;           // request of its first tile
@@ -99,7 +100,7 @@ struct TreePlan {
   int r_n0, r_T, r_ctx, r_len;  // lane i: request i (of the first 32)
   static __device__ __forceinline__ int tiles(const Request &rq) { return (rq.len + TA_KEYS - 1) / TA_KEYS; }
   // what a unit of n tiles takes of the line
-  __device__ __forceinline__ int span(const TreeArgs &a, int n) const { return a.S == 1 ? 1 : n + cost; }
+  static __device__ __forceinline__ int span(const TreeArgs &a, int n) { return a.S == 1 ? 1 : n + TA_UNIT_COST; }
   // units of a KV head
   __device__ __forceinline__ int per_head(const TreeArgs &a, const Request &rq) const {
     return rq.T * a.G <= rows ? 1 : (rq.T * a.G + rows - 1) / rows;
@@ -121,8 +122,8 @@ struct TreePlan {
     return rq;
   }
   // For a whole warp: the stretch of block c of `blocks`.
-  __device__ __forceinline__ TreePlan(const TreeArgs &a, int rows_, int cost_, int blocks, int c)
-      : rows(rows_), cost(cost_), x0(0), count(0), b(a.B), base(0) {
+  __device__ __forceinline__ TreePlan(const TreeArgs &a, int rows_, int blocks, int c)
+      : rows(rows_), x0(0), count(0), b(a.B), base(0) {
     const int lane = threadIdx.x & 31;
     int longest = 1, total = 0, first = 0;
     r_n0 = r_T = r_ctx = r_len = 0;

@@ -15,11 +15,12 @@
 //
 // What bounds it, by the rows a KV head has (bf16, 32 heads over 8 KV heads of 64, pages of 64). Few rows: the cache's
 // bytes. 64 requests x 1 token x 8000 positions: 185 us, 5.7 TB/s, 87 % of the measured copy rate; 32 requests x 16
-// drafts x 500 to 4000 positions: 50 us of which 27 are the stream's, the rest begins and ends units (queries in, first
-// tiles, O out, the join). Many rows: the softmax. 16 requests x 64 drafts x 8000 to 32000 positions: 319 us, 2.1 TB/s and
-// 0.37 PFLOP/s; without its exponentials the same loop takes 243 us, without the softmax 201 us. Two row tiles a block
-// halve the reads of the cache there; with one row tile (at most 128 rows a request) two blocks share an SM and one
-// loads while the other is in its softmax.
+// drafts x 500 to 4000 positions: 44 us, of which 30 at 5.0 TB/s, 4 until the first tile, 5 in the join. Many rows: the
+// softmax. 16 requests x 64 drafts x 8000 to 32000 positions: 305 us, 2.2 TB/s and 0.39 PFLOP/s; without its exponentials
+// the same loop took 243 us of 319, without the softmax 201 us. Two row tiles a block
+// halve the reads of the cache there; with one row tile (at most 128 rows a request) and heads of 64 two blocks share an SM
+// and one loads while the other is in its softmax. Heads of 128: 100 requests x 1 token x 100 to 3000 positions 144 us,
+// 4.4 TB/s.
 //
 // Every wait is bounded (about a second of SM clocks); a wait that gives up sets the device error word that
 // lfm2q_check_device reports, and the block ends without writing its rows.
@@ -181,10 +182,14 @@ template <int D, int PIPE>
 struct TcShape {
   static constexpr int HALVES = D / 64;
   static constexpr int THREADS = 32 * (5 * PIPE + 1);  // per row tile four softmax warps and one that issues MMAs
-  // TMEM columns of a row tile: S0 | S1 | O (| P0 | P1 where there is room; else P lies over its S)
-  static constexpr bool OWN_P = D == 64;
+  // One row tile: two blocks share an SM at D = 64; at D = 128 they would have room for two stages each, and one block with
+  // five is faster (32 requests x 16 drafts 89 -> 84 us, 100 requests x 1 token 158 -> 147).
+  // TMEM columns of a row tile: S0 | S1 | O (| P0 | P1 where there is room, 84 -> 82 us; else P lies over its S)
+  static constexpr bool OWN_P = D == 64 || PIPE == 1;
   static constexpr int O_COL = 2 * TA_KEYS, P_COL = O_COL + D;
-  static constexpr int STAGES = PIPE == 1 ? (D == 64 ? 5 : 2) : (D == 64 ? 8 : 4);
+  static constexpr int TMEM_COLS = PIPE == 1 && D == 64 ? 256 : 512;
+  static constexpr int BLOCKS = PIPE == 1 && D == 64 ? 2 : 1;  // an SM
+  static constexpr int STAGES = PIPE == 1 ? 5 : (D == 64 ? 8 : 4);
   static constexpr int Q_BYTES = HALVES * TT_ATOM;   // per row tile
   static constexpr int KV_BYTES = HALVES * TT_HALF;  // a K (or V) tile
   static constexpr int OUT_BYTES = 2048;             // per softmax warp: 64 bytes of its 32 rows on their way out
@@ -277,14 +282,14 @@ __device__ __noinline__ void add_apart(const TreeArgs &a, unsigned long long ext
 }
 
 template <class T, int D, int PIPE>
-__global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
+__global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, TcShape<D, PIPE>::BLOCKS)
     tree_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                    const __grid_constant__ CUtensorMap tmV, const __grid_constant__ TreeArgs a, int box, int tpt) {
   using L = TcShape<D, PIPE>;
   constexpr int STAGES = L::STAGES, HALVES = L::HALVES;
   constexpr bool BF = std::is_same<T, bf16>::value;
   constexpr int W_TMA = 4 * PIPE, W_MMA = W_TMA + 1;
-  constexpr int TMEM_COLS = 256 * PIPE;
+  constexpr int TMEM_COLS = L::TMEM_COLS;
   extern __shared__ uint8_t tt_smem[];
   __shared__ __align__(8) uint64_t full[STAGES], empty[STAGES], q_full, q_empty, s_full[PIPE][2], p_full[PIPE][2],
       pv_done[PIPE], o_full[PIPE], drained[PIPE];
@@ -337,7 +342,7 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, PIPE == 1 ? 2 : 1)
 
   if (warp == W_TMA) {
     // ---------------------------------------------------------------- segments, queries, K and V tiles
-    const TreePlan plan(a, PIPE * tpt * a.G, unit_cost(D), gridDim.x, blockIdx.x);
+    const TreePlan plan(a, PIPE * tpt * a.G, gridDim.x, blockIdx.x);
     const int boxes = TA_KEYS / box, page_step = TA_KEYS / a.page, row_step = TA_KEYS % a.page;
     int left = plan.count, b = plan.b, base = plan.base, st = 0, ph = 1;  // a fresh barrier passes a wait for phase 1
     // of request b: tiles of a unit, its span on the line, units of a head and in all; the next unit, tile within it
@@ -756,7 +761,7 @@ bool make_map(CUtensorMap *map, const void *ptr, int D, long long y, long long z
 }
 
 template <class T, int D, int PIPE>
-cudaError_t launch(const TreeArgs &a, int blocks, bool pdl, cudaStream_t st) {
+cudaError_t launch(const TreeArgs &a, bool pdl, cudaStream_t st) {
   using L = TcShape<D, PIPE>;
   auto kernel = tree_tc_kernel<T, D, PIPE>;
   static std::atomic<int> attr_set[64];  // the shared-memory opt-in, once per device
@@ -777,23 +782,22 @@ cudaError_t launch(const TreeArgs &a, int blocks, bool pdl, cudaStream_t st) {
       !make_map(&mv, a.vc, D, a.page, heads, box, 1, half))
     return cudaErrorNotSupported;
   cudaLaunchAttribute attr;
-  cudaLaunchConfig_t cfg = pdl_config(dim3(blocks), dim3(L::THREADS), pdl, st, &attr);
+  cudaLaunchConfig_t cfg = pdl_config(dim3(L::BLOCKS * device_sm_count()), dim3(L::THREADS), pdl, st, &attr);
   cfg.dynamicSmemBytes = L::SMEM;
   return cudaLaunchKernelEx(&cfg, kernel, mq, mk, mv, a, box, tpt);
 }
 template <class T, int D>
-cudaError_t launch(const TreeArgs &a, bool pdl, cudaStream_t st) {
-  // Up to 128 rows a request: one row tile a block, two blocks an SM. More: two row tiles a block (they share the K and
-  // V tiles), one block an SM.
-  if (a.max_q <= TT_ROWS / a.G) return launch<T, D, 1>(a, 2 * device_sm_count(), pdl, st);
-  return launch<T, D, 2>(a, device_sm_count(), pdl, st);
+cudaError_t launch_form(const TreeArgs &a, bool pdl, cudaStream_t st) {
+  // Up to 128 rows a request: one row tile a block. More: two row tiles a block, which share the K and V tiles.
+  if (a.max_q <= TT_ROWS / a.G) return launch<T, D, 1>(a, pdl, st);
+  return launch<T, D, 2>(a, pdl, st);
 }
 
 }  // namespace
 
 cudaError_t launch_tree_tc(const TreeArgs &a, int D, bool half, bool pdl, cudaStream_t st) {
-  if (half) return D == 64 ? launch<__half, 64>(a, pdl, st) : launch<__half, 128>(a, pdl, st);
-  return D == 64 ? launch<bf16, 64>(a, pdl, st) : launch<bf16, 128>(a, pdl, st);
+  if (half) return D == 64 ? launch_form<__half, 64>(a, pdl, st) : launch_form<__half, 128>(a, pdl, st);
+  return D == 64 ? launch_form<bf16, 64>(a, pdl, st) : launch_form<bf16, 128>(a, pdl, st);
 }
 
 int tree_device_error(bool clear) {
