@@ -148,7 +148,7 @@ struct TreePlan {
     if (a.S > 1 && (long long)quota * (a.S - 1) < longest) quota = (longest + a.S - 2) / (a.S - 1);
     // A part of few tiles and many rows writes, and the joining kernel reads, more than it loads: a tile for every 64 rows
     // (5 requests x 13 drafts, 104 rows of 128: 21.6 us with a tile a part, 19.3 with two).
-    quota = max(quota, (min(rows, a.max_q * a.G) + 63) / 64);
+    if (a.S > 1) quota = max(quota, (min(rows, a.max_q * a.G) + 63) / 64);
     if ((long long)quota * c >= total) return;
     x0 = quota * c;
     count = min(quota, total - x0);
