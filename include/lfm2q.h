@@ -296,6 +296,17 @@ int lfm2q_sample_next(const void *logits, int dtype, int64_t row_stride, const f
                       const float *top_p, const float *min_p, const float *u, int64_t *tok, int64_t *pos, int B, int V,
                       void *stream);
 
+/* The four operators above from one block of `count` 8-byte words, their arguments in order: pointers and integers as
+ * int64_t, floats as double. For callers that pay by the argument, as ctypes does: 22 arguments take 2.4 us there, one
+ * block of 22 words 0.9. An integer that does not fit its argument is refused. */
+typedef enum {
+  LFM2Q_KV_SLOTS = 0,
+  LFM2Q_QK_NORM_ROPE_KV_PAGED = 1,
+  LFM2Q_TREE_ATTENTION = 2,
+  LFM2Q_SAMPLE_NEXT = 3
+} lfm2q_op;
+int lfm2q_call_words(int op, const void *words, int count);
+
 /* Replace set_pdl / set_gemv_impl (kernels/lfm2_decode.cpp:165-166). set_pdl toggles Programmatic Dependent
  * Launch for the GEMV kernels (default on). set_gemv_impl is accepted for compatibility; this build has one
  * GEMV implementation. */

@@ -9,6 +9,7 @@
 #include <atomic>
 #include <cstdio>
 #include <mutex>
+#include <cstring>
 #include <string>
 #include <vector>
 
@@ -515,6 +516,45 @@ int lfm2q_sample_next(const void *logits, int dtype, int64_t row_stride, const f
   return launched(launch_sample_next(logits, dtype, row_stride, temperature, top_k, top_p, min_p, u, tok, pos, B, V,
                                      g_pdl.load(), (cudaStream_t)stream),
                   "sample_next");
+}
+
+int lfm2q_call_words(int op, const void *words, int count) {
+  // arguments of each entry point, and which of them are int (a bit each)
+  static const struct {
+    int count;
+    uint32_t ints;
+  } ops[] = {{15, 0xfu << 9}, {22, 1u << 5 | 0x7fu << 12 | 1u << 20}, {22, 0x7ffu << 9}, {13, 1u << 1 | 3u << 10}};
+  REQUIRE(op >= 0 && op < (int)(sizeof(ops) / sizeof(ops[0])), "call_words: no such operator");
+  REQUIRE(words && count == ops[op].count, "call_words: the operator has another number of arguments");
+  int64_t w[24];
+  std::memcpy(w, words, (size_t)count * 8);
+  for (int k = 0; k < count; ++k)
+    REQUIRE(!(ops[op].ints >> k & 1) || w[k] == (int32_t)w[k], "call_words: an argument does not fit its 32 bits");
+  const auto p = [&](int k) { return reinterpret_cast<void *>(w[k]); };
+  const auto i = [&](int k) { return (int)w[k]; };
+  const auto f = [&](int k) {
+    double d;
+    std::memcpy(&d, &w[k], 8);
+    return (float)d;
+  };
+  typedef uint16_t u16;
+  typedef int32_t i32;
+  switch (op) {
+    case LFM2Q_KV_SLOTS:
+      return lfm2q_kv_slots((i32 *)p(0), (i32 *)p(1), (i32 *)p(2), (i32 *)p(3), (i32 *)p(4), (i32 *)p(5), (i32 *)p(6),
+                            (int64_t *)p(7), (int64_t *)p(8), i(9), i(10), i(11), i(12), w[13], p(14));
+    case LFM2Q_QK_NORM_ROPE_KV_PAGED:
+      return lfm2q_qk_norm_rope_kv_paged((u16 *)p(0), w[1], (u16 *)p(2), (u16 *)p(3), (float *)p(4), i(5), f(6),
+                                         (int64_t *)p(7), (int64_t *)p(8), (u16 *)p(9), (u16 *)p(10), (u16 *)p(11),
+                                         i(12), i(13), i(14), i(15), i(16), i(17), i(18), f(19), i(20), p(21));
+    case LFM2Q_TREE_ATTENTION:
+      return lfm2q_tree_attention((u16 *)p(0), (u16 *)p(1), (u16 *)p(2), (i32 *)p(3), (i32 *)p(4), (i32 *)p(5),
+                                  (int64_t *)p(6), (u16 *)p(7), (float *)p(8), i(9), i(10), i(11), i(12), i(13), i(14),
+                                  i(15), i(16), i(17), i(18), i(19), f(20), p(21));
+    default:
+      return lfm2q_sample_next(p(0), i(1), w[2], (float *)p(3), (i32 *)p(4), (float *)p(5), (float *)p(6),
+                               (float *)p(7), (int64_t *)p(8), (int64_t *)p(9), i(10), i(11), p(12));
+  }
 }
 
 }  // extern "C"

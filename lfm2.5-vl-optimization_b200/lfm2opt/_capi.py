@@ -5,6 +5,7 @@ Loading fails loudly when the library has not been built: there is no CPU or PyT
 
 import ctypes
 import os
+import struct
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "liblfm2q.so"
@@ -56,6 +57,7 @@ SIGNATURES = {
     "lfm2q_tree_attention": [_p, _p, _p, _p, _p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _i, _f, _p],
     "lfm2q_tree_attention_splits": [_i, _i, _i, _i, _i, _i],
     "lfm2q_sample_next": [_p, _i, _l, _p, _p, _p, _p, _p, _p, _p, _i, _i, _p],
+    "lfm2q_call_words": [_i, _p, _i],
     "lfm2q_decode_attention_split_noalloc": [_p, _p, _p, _p, _p, _i, _i, _i, _i, _i, _f, _p],
 }
 _VOID = {"lfm2q_set_pdl", "lfm2q_set_gemv_impl", "lfm2q_set_gemm_tile", "lfm2q_set_gemv_trigger",
@@ -67,6 +69,12 @@ class GemvLayer(ctypes.Structure):
     """lfm2q_gemv_layer (include/lfm2q.h)."""
 
     _fields_ = [("W", _p), ("scale", _p), ("x", _p), ("y", _p), ("N", _i), ("K", _i)]
+
+# lfm2q_call_words: (operator, layout of its arguments, their number)
+KV_SLOTS = (0, struct.Struct("15q").pack, 15)
+QK_NORM_ROPE_KV_PAGED = (1, struct.Struct("6qd12qd2q").pack, 22)
+TREE_ATTENTION = (2, struct.Struct("20qdq").pack, 22)
+SAMPLE_NEXT = (3, struct.Struct("13q").pack, 13)
 
 _LIB = None
 

@@ -18,6 +18,7 @@ bf16 silu_mul, prefill) are not part of this library; reaching for them raises A
 
 import ctypes
 import os
+import struct
 
 import torch
 
@@ -48,15 +49,18 @@ def _arg(t, dtype, name, dev):
     raise RuntimeError(f"{name}: every tensor must be on one device")
 
 
-def _launch(fn, dev, *args):
-    """Call entry point fn(*args, stream) on PyTorch's current stream of device dev, that device current; raise
-    RuntimeError with the library's message on a non-OK status."""
-    prev = torch._C._cuda_getDevice()
-    if prev != dev:
+def _launch(op, dev, *args):
+    """Call operator op (_capi.KV_SLOTS, ...) with args and PyTorch's current stream of device dev, that device current;
+    raise RuntimeError with the library's message on a non-OK status. A null pointer is 0."""
+    if torch._C._cuda_getDevice() != dev:
         with torch.cuda.device(dev):
-            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+            return _launch(op, dev, *args)
+    code, pack, n = op
+    try:
+        words = pack(*args, torch._C._cuda_getCurrentRawStream(dev))
+    except struct.error as e:
+        raise RuntimeError(f"lfm2q: an argument is not a number of its kind: {e}") from None
+    st = _capi.lib().lfm2q_call_words(code, words, n)
     if st != _capi.OK:
         raise RuntimeError(_capi.lib().lfm2q_last_error().decode() or f"lfm2q: status {st}")
 
@@ -444,7 +448,7 @@ class DecodeGemvExt:
     # -------------------------------------------------- batches of requests over a paged cache (include/lfm2q.h)
     # These are called a few times a decode iteration on small work, so the checks are written to cost little on the
     # host: one helper call a tensor that returns its pointer, messages formed only on failure (17-20 us a call with
-    # the checks above, 8-13 us so, of which the launch is 4-7).
+    # the checks above, 8-13 us so), and the arguments go to the library in one block (7-12 us).
     def kv_slots(self, lens, new_lens, table, free, n_free, page, got, cu, positions, slots):
         """Block tables and slot maps from request lengths (no counterpart in the reference; lfm2q_kv_slots has the
         rules). lens, new_lens, got int32 [B], table int32 [B, max_pages], free int32 [num_pages] with n_free int32 [1]
@@ -460,7 +464,7 @@ class DecodeGemvExt:
             raise RuntimeError("need lens, new_lens, got [B], cu [B + 1], n_free [1]")
         if positions.numel() != capacity:
             raise RuntimeError("positions and slots must have one length")
-        _launch(_capi.lib().lfm2q_kv_slots, dev, *p, B, table.size(1), free.numel(), page, capacity)
+        _launch(_capi.KV_SLOTS, dev, *p, B, table.size(1), free.numel(), page, capacity)
 
     @staticmethod
     def _paged(dtype, kc, vc, name, dev):
@@ -492,14 +496,14 @@ class DecodeGemvExt:
             raise RuntimeError("qkv must be [N, (NQ + 2 NKV) * D]")
         if (qw is None) != (kw is None):
             raise RuntimeError("qw and kw: both or neither")
-        wq = wk = None
+        wq = wk = 0
         if qw is not None:
             wq, wk = _arg(qw, dtype, "qw", dev), _arg(kw, dtype, "kw", dev)
             if qw.numel() != D or kw.numel() != D:
                 raise RuntimeError("qw and kw must be [D]")
         if positions.numel() != N or slots.numel() != N:
             raise RuntimeError("positions and slots must be [N]")
-        _launch(_capi.lib().lfm2q_qk_norm_rope_kv_paged, dev, qkv.data_ptr(), qkv.stride(0) if N > 1 else width, wq,
+        _launch(_capi.QK_NORM_ROPE_KV_PAGED, dev, qkv.data_ptr(), qkv.stride(0) if N > 1 else width, wq,
                 wk, _arg(inv_freq, _F32, "inv_freq", dev), 2 * inv_freq.numel(), scaling,
                 _arg(positions, _I64, "positions", dev), _arg(slots, _I64, "slots", dev), qp, kp, vp, dt, N, NQ, NKV, D,
                 pages, page, eps, 1 if interleaved else 0)
@@ -523,7 +527,7 @@ class DecodeGemvExt:
         N, NQ, _ = shape
         if table.dim() != 2 or table.size(0) != B or cu.numel() != B + 1:
             raise RuntimeError("table must be [B, max_pages] and cu [B + 1]")
-        mp = wp = None
+        mp = wp = 0
         S = 1
         if mask is not None:
             mp = _arg(mask, _I64, "mask", dev)
@@ -534,7 +538,7 @@ class DecodeGemvExt:
             if ws.dim() != 4 or ws.size(0) != N or ws.size(1) != NQ or ws.size(3) != D + 2:
                 raise RuntimeError("ws must be [N, NQ, S, D + 2]")
             S = ws.size(2)
-        _launch(_capi.lib().lfm2q_tree_attention, dev, qp, kp, vp, _arg(table, _I32, "table", dev),
+        _launch(_capi.TREE_ATTENTION, dev, qp, kp, vp, _arg(table, _I32, "table", dev),
                 _arg(ctx, _I32, "ctx", dev), _arg(cu, _I32, "cu", dev), mp, op, wp, dt, N, B, NQ, NKV, D, pages, page,
                 table.size(1), S, max_q, scale)
 
@@ -549,16 +553,16 @@ class DecodeGemvExt:
         p = []
         for t, dtype, name in ((temperature, _F32, "temperature"), (top_k, _I32, "top_k"), (top_p, _F32, "top_p"),
                                (min_p, _F32, "min_p")):
-            p.append(None if t is None else _arg(t, dtype, name, dev))
+            p.append(0 if t is None else _arg(t, dtype, name, dev))
             if t is not None and t.numel() != B:
                 raise RuntimeError(f"{name} must be [B]")
         if u is None or u.numel() != B:
             raise RuntimeError("u: one uniform a row, fp32 [B]")
         if tok.numel() != B:
             raise RuntimeError("tok must be [B]")
-        _launch(_capi.lib().lfm2q_sample_next, dev, logits.data_ptr(), dt, logits.stride(0) if B > 1 else V, *p,
+        _launch(_capi.SAMPLE_NEXT, dev, logits.data_ptr(), dt, logits.stride(0) if B > 1 else V, *p,
                 _arg(u, _F32, "u", dev), _arg(tok, _I64, "tok", dev),
-                None if pos is None else _arg(pos, _I64, "pos", dev), B, V)
+                0 if pos is None else _arg(pos, _I64, "pos", dev), B, V)
 
     def set_pdl(self, on):
         """Enable/disable Programmatic Dependent Launch for the GEMV kernels (default on)."""

@@ -128,3 +128,31 @@ def test_plain_forms_agree_with_direct_ones():
     p = np.exp(x - x.max())
     assert sample_next_f64(x, 1.0, 0, 1.0, 0.0, 0.5) == int(np.searchsorted(np.cumsum(p), 0.5 * p.sum(), side="right"))
     assert sample_next_f64(x, 1.0, 1, 1.0, 0.0, 0.99) == int(x.argmax())
+
+
+@pytest.mark.skipif(torch.cuda.is_available(), reason="some of the calls are valid but for their pointers")
+def test_arguments_in_one_block():
+    """lfm2q_call_words: the same answer as the entry point for each operator, and its own refusals."""
+    L = _capi.lib()
+    calls = {_capi.KV_SLOTS: ("lfm2q_kv_slots", [F, F + 64, F, F, F, F + 128, F, F, F, 4, 8, 100, 16, 64, 0], 12),
+             _capi.QK_NORM_ROPE_KV_PAGED: ("lfm2q_qk_norm_rope_kv_paged",
+                                           [F, 1024, F, F, F, 64, 1.0, F, F, F, F, F, _capi.BF16, 4, 8, 4, 64, 10, 16,
+                                            1e-5, 0, 0], 5),
+             _capi.TREE_ATTENTION: ("lfm2q_tree_attention",
+                                    [F] * 9 + [_capi.BF16, 20, 2, 8, 2, 64, 10, 16, 8, 2, 10, 0.125, 0], 19),
+             _capi.SAMPLE_NEXT: ("lfm2q_sample_next", [F, _capi.BF16, 1000, 0, 0, 0, 0, F, F, 0, 2, 1000, 0], 11)}
+    for (code, pack, n), (name, ok, number) in calls.items():
+        assert len(ok) == n == len(_capi.SIGNATURES[name])
+        kinds = [type(v) for v in ok]
+        for k in range(n):  # every argument in its place: a bad value of each is answered alike
+            for bad in ((-1.0, float("nan")) if kinds[k] is float else (0, 7, -5)):
+                a = swap(ok, **{f"_{k}": bad})
+                st = getattr(L, name)(*[None if v == 0 and t is _capi._p else v
+                                        for v, t in zip(a, _capi.SIGNATURES[name])])
+                said = L.lfm2q_last_error()
+                assert L.lfm2q_call_words(code, pack(*a), n) == st, (name, k, bad)
+                assert L.lfm2q_last_error() == said, (name, k, bad)
+        refused("lfm2q_call_words", (code, pack(*ok), n - 1), "number of arguments")
+        refused("lfm2q_call_words", (code, pack(*swap(ok, **{f"_{number}": 1 << 32})), n), "32 bits")
+    refused("lfm2q_call_words", (4, bytes(8 * 24), 13), "no such operator")
+    refused("lfm2q_call_words", (0, None, 15), "number of arguments")
