@@ -178,3 +178,20 @@ def test_spreads(cuda_dev, scale):
     p = params(np.random.default_rng(8), 30)
     p["temperature"] = [1.0] * 30
     assert draw(cuda_dev, x, **p) == want(x, **p)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("k", [2, 3, 31, 100, 127, 128, 129, 130, 300])
+def test_lists_on_both_sides_of_the_pairwise_limit(cuda_dev, k, dt):
+    """top_k around 128, with ties across the cut (equal logits at the k-th place) and without, each filter on and off."""
+    g = torch.Generator().manual_seed(k)
+    B, V = 24, 30011
+    x = 2.0 * torch.randn(B, V, generator=g)
+    x[::3] = (x[::3] * 4).round() / 4  # many equal logits
+    x = x.to(DT[dt])
+    rng = np.random.default_rng(k)
+    pick = lambda *a: [a[i % len(a)] for i in range(B)]  # noqa: E731
+    p = dict(temperature=pick(0.5, 1.0, 1.0, 2.0, 1e-4), top_k=[k] * B, top_p=pick(1.0, 0.9, 0.3, 0.99),
+             min_p=pick(0.0, 0.0, 0.2, 0.0, 0.01), u=rng.random(B, dtype=np.float32).tolist())
+    p["u"][:2] = [0.0, float(np.nextafter(np.float32(1), np.float32(0)))]
+    assert draw(cuda_dev, x, **p) == want(x, **p)

@@ -292,3 +292,36 @@ def test_two_streams_at_once(cuda_dev):
     for c, ref, (_, _, out, _) in zip(cs, refs, work):
         check(out, ref, c)
     check_device()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16"])
+@pytest.mark.parametrize("NQ,T", [(8, 1), (8, 3), (32, 16), (32, 64)])
+def test_long_units_of_wide_heads(cuda_dev, NQ, T, dt):
+    """Heads of 128: more tiles than stages in one block, one row tile and two, units cut in parts of many lengths."""
+    c = make(40 + T, NQ, NQ // 4, 128, 32, [3000, 70], [T, T], dt)
+    for S in (None, 1, 2, 9):
+        check(run(cuda_dev, c, S), reference(c), c)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_many_units_in_a_block(cuda_dev, D):
+    """More units than blocks have stretches: several units, whole and cut ones, follow each other in a block."""
+    rng = np.random.default_rng(D)
+    ctx, T = rng.integers(0, 400, 260).tolist(), rng.integers(1, 3, 260).tolist()
+    c = make(14, 16, 4, D, 64, ctx, T, "bf16")
+    for S in (1, 2, 4):
+        check(run(cuda_dev, c, S), reference(c), c)
+
+
+def test_other_workspaces_contents_do_not_matter(cuda_dev):
+    """The joining kernel reads what this call's parts wrote: the same bits over any contents of the workspace."""
+    c = make(15, 32, 8, 64, 64, [1500, 200, 40], [5, 16, 1], "bf16")
+    d = {k: v.to(cuda_dev) for k, v in c.items() if torch.is_tensor(v)}
+    outs = []
+    for fill in (0.0, 1e30, float("inf"), -1.0):
+        out, ws = torch.zeros_like(d["q"]), torch.full((22, 32, 20, 66), fill, device=cuda_dev)
+        ext().tree_attention(d["q"], d["kc"], d["vc"], d["table"], d["ctx"], d["cu"], signed(c["mask"]).to(cuda_dev), out,
+                             ws, c["scale"], 16)
+        outs.append(out.cpu())
+    check(outs[0], reference(c), c)
+    assert all(torch.equal(outs[0], o) for o in outs[1:])
