@@ -21,8 +21,8 @@
 // What bounds it: a pass over the staged row costs about 10 (counts) to 30 (weights in fp64) issue slots an element,
 // against 2 to 4 bytes to load; the cluster's four barriers and the sort are latency, some microseconds a row. Rows of
 // 65536: 256 in fp32 take 117 us with a nucleus alone (0.57 TB/s; two blocks an SM issue 2.2 instructions a clock and the
-// fp64 pipe is 18 % busy), in bf16 62 us unfiltered and 43 us with a top_k of 50 (no fp64 pass over the row); one row in
-// bf16 10.5 us. The list replaces an exact histogram over the whole row, several passes (16 rows with a top_k of 5000,
+// fp64 pipe is 18 % busy), in bf16 62 us unfiltered and 40 us with a top_k of 50 (no fp64 pass over the row); one row in
+// bf16 10.4 us. The list replaces an exact histogram over the whole row, several passes (16 rows with a top_k of 5000,
 // which still take them: 70 us). The other blocks leave before the list is sorted, so the next row starts on their SMs
 // (124 -> 120 us), and the whole block searches the piece that holds the token (120 -> 117; a warp did it before).
 #include <cooperative_groups.h>
@@ -150,6 +150,13 @@ struct SampleShared {
   };
 };
 
+// adds v to a word of shared memory, OFF bytes from addr, where `in`; without a branch (64 rows with a top_k of 100: 20.0 us
+// with branches, 18.6 so)
+template <int OFF>
+__device__ __forceinline__ void add_if(bool in, uint32_t addr, uint32_t v) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %0, 0;\n\t@p red.shared.add.u32 [%1 + %3], %2;\n\t}" ::"r"((int)in),
+               "r"(addr), "r"(v), "n"(OFF));  // (no clobber: loads may pass it, the barriers do not)
+}
 __device__ __forceinline__ unsigned long long shfl_up64(unsigned long long v, int o) {
   return __shfl_up_sync(0xffffffffu, v, o);
 }
@@ -188,7 +195,7 @@ struct Weigher {
 };
 // Level 0 bins: linear in x, monotone, bin i around 2^(-46 i / 1024) of the largest weight; the last one takes all that
 // weighs less than 2^-46. The maximum is finite. place() + 2^23 rounds to the bin, its low bits.
-constexpr float SA_RND = 8388608.f;
+constexpr float SA_RND = 8388608.f, SA_TO_INT = 12582912.f;
 struct Binner {
   float mx, scale;
   __device__ __forceinline__ float place(float f) const { return (mx - f) * scale; }
@@ -784,21 +791,19 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
   // times infinity: an infinite maximum, a temperature near 0 (every block finds the same)
   bool again = best == INFINITY || !(bins.scale < 1e30f);
   if ((use_k || use_p) && !again) {
+    const uint32_t cnt0 = (uint32_t)__cvta_generic_to_shared(s.f.cnt) - 4 * __float_as_uint(SA_RND);
     for (int v = w0 + lane; v < w1; v += 32) {
       const uint4 q = stage[v];
       const raw *qr = reinterpret_cast<const raw *>(&q);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const float d = bins.place(E::up(qr[j]));
-        if (d < (float)(SA_BINS - 2)) {  // (a filler is a NaN)
-          const float rnd = d + SA_RND;
-          const int bin = __float_as_int(rnd) - __float_as_int(SA_RND);
-          atomicAdd(&s.f.cnt[bin], 1u);
-          // the offset from the middle times 2^12, to an integer by adding 1.5 2^23
-          if (!use_k)
-            atomicAdd(&s.f.frac[bin], __float_as_int(fmaf(d - (rnd - SA_RND), 4096.f, 12582912.f)) -
-                                          __float_as_int(12582912.f));
-        }
+        const float d = bins.place(E::up(qr[j])), rnd = d + SA_RND;
+        const bool in = d < (float)(SA_BINS - 2);  // (a filler is a NaN)
+        const uint32_t cnt = cnt0 + 4 * __float_as_uint(rnd);
+        add_if<0>(in, cnt, 1);
+        // the offset from the middle times 2^12, to an integer by adding 1.5 2^23, whose bits go once the counts are known
+        if (!use_k)
+          add_if<sizeof(s.f.cnt)>(in, cnt, __float_as_uint(fmaf(d - (rnd - SA_RND), 4096.f, SA_TO_INT)));
       }
     }
     cl.sync();
@@ -822,6 +827,8 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
         fr[0] += w[c].x;
         fr[1] += w[c].y;
       }
+      fr[0] -= n[0] * __float_as_uint(SA_TO_INT);  // (modulo 2^32; the sums themselves fit)
+      fr[1] -= n[1] * __float_as_uint(SA_TO_INT);
     }
     constexpr float H = 0.69314718f * 46.f / SA_BINS;
     float m[2];
