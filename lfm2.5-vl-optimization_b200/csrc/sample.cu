@@ -194,14 +194,18 @@ struct Weigher {
   }
 };
 // Level 0 bins: linear in x, monotone, bin i around 2^(-46 i / 1024) of the largest weight; the last one takes all that
-// weighs less than 2^-46. The maximum is finite. place() + 2^23 rounds to the bin, its low bits.
+// weighs less than 2^-45.9. The maximum is finite. place() + 2^23 rounds to the bin, its low bits. Which bin an element
+// falls into, and whether it falls into one before the last, is decided here alone: the list is sized by counts of the
+// one pass and filled by the next, which therefore has to see the same bins.
 constexpr float SA_RND = 8388608.f, SA_TO_INT = 12582912.f;
 struct Binner {
   float mx, scale;
   __device__ __forceinline__ float place(float f) const { return (mx - f) * scale; }
+  __device__ __forceinline__ float rounded(float f) const { return place(f) + SA_RND; }  // 2^23 + bin
+  static __device__ __forceinline__ bool early(float rnd) { return rnd < SA_RND + (float)(SA_BINS - 1); }  // (no NaN)
   __device__ __forceinline__ int operator()(float f) const {
-    const float d = place(f);
-    return d < (float)(SA_BINS - 2) ? __float_as_int(d + SA_RND) - __float_as_int(SA_RND) : SA_BINS - 1;
+    const float rnd = rounded(f);
+    return early(rnd) ? __float_as_int(rnd) - __float_as_int(SA_RND) : SA_BINS - 1;
   }
 };
 // What a block of the cluster has of the row.
@@ -787,6 +791,7 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
 
   // ---------------------------------------------------------------- where the cut lies: bins [b_lo, b_hi]
   int b_lo = SA_BINS, b_hi = -1;  // no cut: everything is "above"
+  uint32_t held = 0;              // elements in them
   // the exact histograms where the list would be too long, or where the bins and the branch-free weights would meet 0
   // times infinity: an infinite maximum, a temperature near 0 (every block finds the same)
   bool again = best == INFINITY || !(bins.scale < 1e30f);
@@ -797,8 +802,8 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
       const raw *qr = reinterpret_cast<const raw *>(&q);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const float d = bins.place(E::up(qr[j])), rnd = d + SA_RND;
-        const bool in = d < (float)(SA_BINS - 2);  // (a filler is a NaN)
+        const float d = bins.place(E::up(qr[j])), rnd = bins.rounded(E::up(qr[j]));
+        const bool in = Binner::early(rnd);  // (a filler is a NaN)
         const uint32_t cnt = cnt0 + 4 * __float_as_uint(rnd);
         add_if<0>(in, cnt, 1);
         // the offset from the middle times 2^12, to an integer by adding 1.5 2^23, whose bits go once the counts are known
@@ -882,14 +887,16 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
     if (use_k) {
       b_lo = 0;
       b_hi = at;
-      again = at == SA_BINS - 1 || s.f.cum[at] > SA_LIST;
+      held = s.f.cum[at];
+      again = at == SA_BINS - 1 || held > SA_LIST;
     } else {
       b_lo = max(0, at - (s.bin >> 16 & 1));
       b_hi = min(SA_BINS - 2, at + (s.bin >> 17 & 1));
       // (an empty neighbour holds nothing that could be cut: the next one with elements does)
       while (s.bin >> 16 & 1 && b_lo > 0 && s.f.cum[b_lo] == s.f.cum[b_lo - 1]) --b_lo;
       while (s.bin >> 17 & 1 && b_hi < SA_BINS - 2 && s.f.cum[b_hi] == s.f.cum[b_hi - 1]) ++b_hi;
-      again = b_hi < b_lo || s.f.cum[b_hi] - (b_lo ? s.f.cum[b_lo - 1] : 0u) > SA_LIST;
+      held = s.f.cum[b_hi] - (b_lo ? s.f.cum[b_lo - 1] : 0u);
+      again = b_hi < b_lo || held > SA_LIST;
     }
   }
 
@@ -911,7 +918,7 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < 8; ++j) {  // (a filler is a NaN: it weighs nothing and lies in no bin)
-        const float rnd = bins.place(f[j]) + SA_RND;
+        const float rnd = bins.rounded(f[j]);
         if (rnd >= r_lo && rnd <= r_hi) listed |= 1u << j;
       }
       if (!use_k) {
@@ -922,7 +929,7 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
         for (int j = 0; j < 8; ++j) {
           const unsigned long long wf = Weigher::fixed(w[j]);
           all += wf;
-          if (bins.place(f[j]) + SA_RND < r_lo) {
+          if (bins.rounded(f[j]) < r_lo) {
             above += wf;
             if (mp > 0.0 && w[j] >= mp) kept += wf;
           }
@@ -931,8 +938,10 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
       for (; listed; listed &= listed - 1) {
         const int j = __ffs(listed) - 1, v = vb + 32 * (j / PER), k = j % PER;
         const raw x0 = reinterpret_cast<const raw *>(&stage[v])[k];
-        s.f.key[atomicAdd(&s.n_list, 1)] = (unsigned long long)key_of<E>(x0) << SA_IDX_BITS |
-                                          (unsigned)((1 << SA_IDX_BITS) - 1 - ((v0 + v) * PER - skew + k));
+        const int slot = atomicAdd(&s.n_list, 1);
+        if (slot < SA_LIST)  // (the counts say so too)
+          s.f.key[slot] = (unsigned long long)key_of<E>(x0) << SA_IDX_BITS |
+                          (unsigned)((1 << SA_IDX_BITS) - 1 - ((v0 + v) * PER - skew + k));
       }
     }
     if (mp == 0.0) kept = above;
@@ -978,6 +987,11 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
           n += nc;
         }
       }
+      const bool whole = n == (int)held;  // the list holds what was counted
+      if (!whole) {
+        n = 0;
+        if (t < C) cl.map_shared_rank(&s, t)->again = 1;
+      }
       for (int i = t; i < n; i += SA_T) {
         int c = 0;
 #pragma unroll
@@ -991,7 +1005,7 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
       }
       if (t == 0) s.cut = 0;
       __syncthreads();
-      if (use_p && !use_k) {  // does the cut lie in the list?
+      if (whole && use_p && !use_k) {  // does the cut lie in the list?
         unsigned long long sum = 0, before, total;
         for (int i = t; i < n; i += SA_T)
           sum += Weigher::fixed(weigh(value_of<E>((uint32_t)(s.f.key[i] >> SA_IDX_BITS))));

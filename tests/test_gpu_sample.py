@@ -195,3 +195,22 @@ def test_lists_on_both_sides_of_the_pairwise_limit(cuda_dev, k, dt):
              min_p=pick(0.0, 0.0, 0.2, 0.0, 0.01), u=rng.random(B, dtype=np.float32).tolist())
     p["u"][:2] = [0.0, float(np.nextafter(np.float32(1), np.float32(0)))]
     assert draw(cuda_dev, x, **p) == want(x, **p)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("B,V", [(1, 65536), (20, 5000), (200, 65536)])
+def test_flat_tails_at_the_last_bins(cuda_dev, B, V, dt):
+    """Thousands of equal logits 45.9 binary orders below the largest (1022 of 1024 bins, 46 orders in all), where the
+    counted elements end, with a top_k or a nucleus whose cut lies there: what is counted is what is listed."""
+    bins = 1024 / (46 * np.log(2))  # bins a unit of logits at temperature 1
+    places = (1020.6, 1021.4, 1021.6, 1021.9, 1022.1, 1022.4, 1022.6, 1023.4)
+    x = torch.full((B, V), -64.0)
+    x[:, 0] = 0.0
+    x[1::2, V // 2] = -63.97  # half a bin above the others, where the type holds it
+    p = dict(temperature=[float(64.0 * bins / places[b % 8]) for b in range(B)],
+             top_k=[(0, 2, 0, 3, 0, 2, 2000)[b % 7] for b in range(B)],
+             top_p=[(1 - 2**-18, 1.0, 0.99999, 0.999999, 1 - 2**-20)[b % 5] for b in range(B)],
+             min_p=[0.0] * B, u=[(0.3, 0.999999, 1.0, 0.0)[b % 4] for b in range(B)])
+    if B == 1:
+        p.update(top_p=[0.99999], temperature=[float(64.0 * bins / 1022.2)])
+    assert draw(cuda_dev, x.to(DT[dt]), **p) == want(x.to(DT[dt]), **p)
