@@ -194,14 +194,17 @@ struct Weigher {
   }
 };
 // Level 0 bins: linear in x, monotone, bin i around 2^(-46 i / 1024) of the largest weight; the last one takes all that
-// weighs less than 2^-45.9. The maximum is finite. place() + 2^23 rounds to the bin, its low bits. Which bin an element
-// falls into, and whether it falls into one before the last, is decided here alone: the list is sized by counts of the
-// one pass and filled by the next, which therefore has to see the same bins.
+// weighs less than 2^-45.9. The maximum is finite. The place on that line plus 2^23 rounds to the bin, its low bits. Which
+// bin an element falls into, and whether it is one before the last, is decided here alone: the list is sized by the counts
+// of one pass and filled by the next, which has to see the same bins.
 constexpr float SA_RND = 8388608.f, SA_TO_INT = 12582912.f;
 struct Binner {
   float mx, scale;
-  __device__ __forceinline__ float place(float f) const { return (mx - f) * scale; }
-  __device__ __forceinline__ float rounded(float f) const { return place(f) + SA_RND; }  // 2^23 + bin
+  // 2^23 + bin. The roundings are spelt out, for the compiler may fuse a * b + c in one place and not in another, which
+  // moves an element next to a bin's edge.
+  __device__ __forceinline__ float rounded(float f) const { return __fmaf_rn(__fsub_rn(mx, f), scale, SA_RND); }
+  // how far f lies from the middle of its bin, in bins
+  __device__ __forceinline__ float off(float f, float rnd) const { return fmaf(mx - f, scale, SA_RND - rnd); }
   static __device__ __forceinline__ bool early(float rnd) { return rnd < SA_RND + (float)(SA_BINS - 1); }  // (no NaN)
   __device__ __forceinline__ int operator()(float f) const {
     const float rnd = rounded(f);
@@ -802,13 +805,13 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
       const raw *qr = reinterpret_cast<const raw *>(&q);
 #pragma unroll
       for (int j = 0; j < PER; ++j) {
-        const float d = bins.place(E::up(qr[j])), rnd = bins.rounded(E::up(qr[j]));
+        const float f = E::up(qr[j]), rnd = bins.rounded(f);
         const bool in = Binner::early(rnd);  // (a filler is a NaN)
         const uint32_t cnt = cnt0 + 4 * __float_as_uint(rnd);
         add_if<0>(in, cnt, 1);
         // the offset from the middle times 2^12, to an integer by adding 1.5 2^23, whose bits go once the counts are known
         if (!use_k)
-          add_if<sizeof(s.f.cnt)>(in, cnt, __float_as_uint(fmaf(d - (rnd - SA_RND), 4096.f, SA_TO_INT)));
+          add_if<sizeof(s.f.cnt)>(in, cnt, __float_as_uint(fmaf(bins.off(f, rnd), 4096.f, SA_TO_INT)));
       }
     }
     cl.sync();

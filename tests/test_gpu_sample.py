@@ -214,3 +214,28 @@ def test_flat_tails_at_the_last_bins(cuda_dev, B, V, dt):
     if B == 1:
         p.update(top_p=[0.99999], temperature=[float(64.0 * bins / 1022.2)])
     assert draw(cuda_dev, x.to(DT[dt]), **p) == want(x.to(DT[dt]), **p)
+
+
+@pytest.mark.parametrize("ties", [60, 1500])
+def test_ties_between_two_bins(cuda_dev, ties):
+    """Equal logits whose place lies so near the border of two of the 1024 bins that it depends on whether a product is
+    rounded before a sum: every pass puts them into the same one, so the cut's list is complete."""
+    f = np.float32
+    scale = f(f(np.log2(np.e) * 1024 / 46))
+    v = np.random.default_rng(0).uniform(1.0, 20.0, 1 << 22).astype(f)
+    place = (v * scale).astype(f)
+    once = (v.astype(np.float64) * np.float64(scale) + 2.0**23).astype(f)  # the product unrounded
+    v = v[once != (place + f(2.0**23)).astype(f)][:40]
+    assert len(v) == 40
+    g = torch.Generator().manual_seed(ties)
+    x = -24.0 - torch.rand(len(v), 5000, generator=g)
+    x[:, 100:120] = -torch.rand(len(v), 20, generator=g)
+    x[:, 7] = 0.0
+    x[:, 2000:2000 + ties] = -torch.from_numpy(v)[:, None]
+    rng = np.random.default_rng(ties)
+    B = len(v)
+    p = dict(temperature=[1.0] * B, top_k=[(0, 50, 22, 21 + ties)[b % 4] for b in range(B)],
+             top_p=[(0.9, 1.0, 0.99999, 1.0, 0.5)[b % 5] for b in range(B)], min_p=[0.0] * B,
+             u=rng.random(B, dtype=f).tolist())
+    p["u"][::3] = [0.99999] * len(p["u"][::3])
+    assert draw(cuda_dev, x, **p) == want(x, **p)
