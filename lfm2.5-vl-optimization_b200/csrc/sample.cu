@@ -906,6 +906,7 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
   if (!again) {
     // -------------------------------------------------------------- weights above the list, and the list
     unsigned long long all = 0, above = 0, kept = 0;
+    const bool no_cut = !(use_k || use_p);
     const float r_lo = SA_RND + (float)b_lo, r_hi = SA_RND + (float)b_hi;
     constexpr int UN2 = 8 / PER;  // eight elements a step
     for (int vb = w0 + lane; vb < w1; vb += 32 * UN2) {
@@ -932,7 +933,8 @@ __global__ void __launch_bounds__(SA_T, 2) sample_kernel(const SampleArgs a) {
         for (int j = 0; j < 8; ++j) {
           const unsigned long long wf = Weigher::fixed(w[j]);
           all += wf;
-          if (bins.rounded(f[j]) < r_lo) {
+          // (without a cut no bin is asked: a difference beyond the largest float has none, and may weigh something)
+          if (no_cut || bins.rounded(f[j]) < r_lo) {
             above += wf;
             if (mp > 0.0 && w[j] >= mp) kept += wf;
           }

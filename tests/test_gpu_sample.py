@@ -239,3 +239,18 @@ def test_ties_between_two_bins(cuda_dev, ties):
              u=rng.random(B, dtype=f).tolist())
     p["u"][::3] = [0.99999] * len(p["u"][::3])
     assert draw(cuda_dev, x, **p) == want(x, **p)
+
+
+def test_spreads_past_the_largest_float(cuda_dev):
+    """Differences of fp32 logits beyond 3.4e38, at temperatures where they still weigh."""
+    g = torch.Generator().manual_seed(9)
+    base = 3.4e38 * (2 * torch.rand(3000, generator=g) - 1)
+    rows, p = [], dict(temperature=[], top_k=[], top_p=[], min_p=[], u=[])
+    for T in (1e37, 1e38, 3.4e38, float("inf")):
+        for k, tp, mp in ((0, 1.0, 0.0), (0, 1.0, 0.2), (0, 0.9, 0.0), (0, 0.5, 0.1), (2000, 1.0, 0.0), (50, 0.9, 0.0)):
+            for u in (0.0, 0.3, 0.6, 0.999):
+                rows.append(base)
+                for n, v in zip(p, (T, k, tp, mp, u)):
+                    p[n].append(v)
+    x = torch.stack(rows)
+    assert draw(cuda_dev, x, **p) == want(x, **p)
