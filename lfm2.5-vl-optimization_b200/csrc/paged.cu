@@ -22,10 +22,10 @@ namespace {
 // a time, the page moves one warp a request. The kernel is latency, a chain of dependent loads (lengths, free pages,
 // table) and barriers, so: the second scan (offsets without the refused requests) and the one of returned pages run only
 // where there are such, the search for a token's request runs in shared memory, and a small batch takes a small block.
-// Sums saturate at 2^30 (every limit is lower), so 32 bits hold them. 37 requests x 16 tokens and the removal of those
-// that were not accepted (two calls, 11 KB): 9.8 us; 64 requests x 1024 tokens (1.1 MB; a second kernel over the whole
-// device writes the rows where there may be more than SL_FILL): 14 us for the two calls.
-constexpr uint32_t SL_MAX = 1u << 30;
+// Sums saturate at 2^31 - 1, past every limit (2^30 at most), and two of them add up within 32 bits. 37 requests x 16 tokens
+// and the removal of those that were not accepted (two calls, 11 KB): 9.8 us; 64 requests x 1024 tokens (1.1 MB; a second
+// kernel over the whole device writes the rows where there may be more than SL_FILL): 14 us for the two calls.
+constexpr uint32_t SL_MAX = 0x7fffffffu;
 constexpr int SL_BIG = 1024;     // threads for batches of more than 256 requests
 constexpr int SL_FILL = 4096;    // token rows that the block fills itself
 

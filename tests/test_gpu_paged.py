@@ -93,6 +93,29 @@ def test_kv_slots_empty_batch_and_refused_requests(cuda_dev):
     assert int(cu) == 0 and int(p.d_n) == p.n_free
 
 
+@pytest.mark.parametrize("each,got", [(1 << 29, [1 << 29, 1 << 29, 0, 0]), ((1 << 29) + 1, [(1 << 29) + 1, 0, 0, 0])])
+def test_kv_slots_at_the_largest_capacity(cuda_dev, each, got):
+    """2^30 token rows (16 GB): two requests that fill them to the last, and two that together bring two more."""
+    page, cap = 1 << 20, 1 << 30
+    i32 = lambda a: torch.tensor(a, dtype=torch.int32, device=cuda_dev)  # noqa: E731
+    table = torch.full((4, 1024), -1, dtype=torch.int32, device=cuda_dev)
+    free, n_free = torch.arange(1500, dtype=torch.int32, device=cuda_dev), i32([1500])
+    d_got, cu = i32([-7] * 4), i32([-7] * 5)
+    pos, slots = [torch.full((cap,), -7, dtype=torch.int64, device=cuda_dev) for _ in range(2)]
+    ext().kv_slots(i32([0] * 4), i32([each, each, 5, 0]), table, free, n_free, page, d_got, cu, pos, slots)
+    cut = np.cumsum([0] + got)
+    assert d_got.tolist() == got and cu.tolist() == cut.tolist()
+    pages = [-(-g // page) for g in got]
+    assert int(n_free) == 1500 - sum(pages) and [int((r >= 0).sum()) for r in table] == pages
+    for b, n in enumerate(got):
+        for t0 in range(0, n, 1 << 28):  # in pieces: a comparison makes several copies
+            t = torch.arange(t0, min(n, t0 + (1 << 28)), device=cuda_dev)
+            at = slice(int(cut[b]) + t0, int(cut[b]) + t0 + len(t))
+            assert torch.equal(pos[at], t)
+            assert torch.equal(slots[at], table[b, t // page].long() * page + t % page)
+    assert (pos[cut[-1]:] == -7).all() and (slots[cut[-1]:] == -7).all()
+
+
 # ---------------------------------------------------------------------------------------------------- rotary positions
 @pytest.mark.parametrize("N,NQ,NKV,D,rot,inter,norm,dt,page,far,kind", [
     (1, 32, 8, 64, 64, False, True, "bf16", 64, 4000, "plain"),
