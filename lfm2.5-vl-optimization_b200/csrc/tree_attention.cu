@@ -7,8 +7,10 @@
 // Mathematics: the rows of one (request, KV head) are its T_b G queries, so K and V are read once for all of them;
 // the online softmax keeps a running maximum m and sum l per row in fp32 (base 2: scores times scale log2 e) and
 // rescales the fp32 accumulator when m grows. The probabilities are rounded to the cache's type for the second
-// product, and l sums the unrounded ones: each p is off by at most half a step, which leaves out within one rounding
-// of that type.
+// product, which 16-bit operands of the tensor cores ask for, and l sums the unrounded ones: each p is off by at most half
+// a step, which leaves out within one rounding of that type. In fp16, whose steps are fixed below 2^-14, they are raised
+// by a power of two before the rounding (here 2^15, and m stands for the maximum less 15): half a step of each holds down
+// to 2^-29 of the largest, and below that each is off by 2^-40 at most (tree_attention_tc.cu: 2^-25 and 2^-36).
 //
 // Two kernels: tree_attention_tc.cu has the one for pages that are multiples of 8 positions (a TMA box of rows never
 // crosses a page, and eight rows are the swizzle's period); this file the one for other pages, and the join of both.
@@ -28,6 +30,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cstdint>
+#include <type_traits>
 
 #include "common.cuh"
 #include "launch.h"
@@ -85,6 +88,7 @@ __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
   constexpr int KW = TA_KEYS / WK;       // keys of a tile per warp
   constexpr int NB = KW / 8;             // 8-key column blocks per warp
   constexpr int TILE = TA_KEYS * D * 2;  // bytes of a K (or V) tile
+  constexpr float RAISE = std::is_same<T, __half>::value ? 15.f : 0.f;
   extern __shared__ __align__(128) uint8_t ta_smem[];
   __shared__ int bad_pages;  // a page outside the pool was met
   __shared__ int red;
@@ -228,7 +232,7 @@ __global__ void __launch_bounds__(32 * WM * WK) tree_kernel(const TreeArgs a) {
         for (int j = 0; j < NB; ++j) mx = fmaxf(mx, fmaxf(s[mt][j][2 * h], s[mt][j][2 * h + 1]));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
         mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-        const float mn = fmaxf(m[mt][h], mx * a.scale_log2);
+        const float mn = fmaxf(m[mt][h], mx * a.scale_log2 - RAISE);
         const float ms = mn == -INFINITY ? 0.f : mn;
         const float corr = ex2(m[mt][h] - ms);  // 2^-inf = 0 while nothing was seen
         m[mt][h] = mn;

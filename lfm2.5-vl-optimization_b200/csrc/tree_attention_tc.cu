@@ -10,8 +10,8 @@
 // MN-major operand); four warps do the softmax, one thread a row, so that a row's maximum and sum need no exchange
 // between lanes. While tile n is in the softmax, S of tile n + 1 is ready, S of tile n + 2 follows as soon as tile n is
 // read, and O of tile n - 1 is accumulated. O stays in TMEM; it is rescaled only when a row's maximum has grown by more
-// than 2^8 since the last time (the probabilities then reach at most 2^8, as exact as below 1), rarely after the first
-// tiles.
+// than 2^8 since the last time (2^4 for fp16; the probabilities then reach at most 2^8, or 2^15 as fp16's are raised by
+// 2^11, as exact as below 1), rarely after the first tiles.
 //
 // What bounds it, by the rows a KV head has (bf16, 32 heads over 8 KV heads of 64, pages of 64). Few rows: the cache's
 // bytes. 64 requests x 1 token x 8000 positions: 185 us, 5.7 TB/s, 87 % of the measured copy rate; 32 requests x 16
@@ -45,7 +45,18 @@ constexpr int TT_ROWS = 128;
 constexpr int TT_ATOM = TT_ROWS * 128;         // 64 dims of the query tile
 constexpr int TT_HALF = TA_KEYS * 128;         // 64 dims of a K (or V) tile
 constexpr long long TT_WAIT_LIMIT = 1ll << 31;
-constexpr float TT_SLACK = 8.f;                // log2 of what a row's maximum may grow before O is rescaled
+// What a row's maximum may grow before O is rescaled, and how far the probabilities are raised, both in log2. fp16 ends at
+// 2^16 and has fixed steps below 2^-14: raised by 11, a probability keeps its 11 bits down to 2^-25 of the largest, and is
+// off by at most 2^-36 below that (unraised 2^-25: 32000 keys of 2^-25 each under one of 1 came out as none, 9e-4 of the
+// result). bf16 has fp32's exponents.
+template <class T>
+struct Range {
+  static constexpr float SLACK = 8.f, RAISE = 0.f;
+};
+template <>
+struct Range<__half> {
+  static constexpr float SLACK = 4.f, RAISE = 11.f;
+};
 
 __device__ __forceinline__ uint32_t smem_addr(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
@@ -552,7 +563,7 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, TcShape<D, PIPE>::B
         const int tok = tok0 + my_tok;
         see = a.mask ? __ldcg(a.mask + g->n0 + tok) : (tok >= 63 ? ~0ull : (2ull << tok) - 1);
       }
-      float m = -INFINITY, l = 0.f;
+      float m = -INFINITY, l = 0.f;  // m: the maximum less what the probabilities are raised by
       for (int n = 0; n < tiles; ++n, ++cnt) {
         const uint32_t sbuf = tbase + (cnt & 1) * TA_KEYS;
         const uint32_t pbuf = L::OWN_P ? tbase + L::P_COL + (cnt & 1) * (TA_KEYS / 2) : sbuf;
@@ -610,13 +621,13 @@ __global__ void __launch_bounds__(TcShape<D, PIPE>::THREADS, TcShape<D, PIPE>::B
             return fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * a.scale_log2;
           };
           // (a unit's first tile starts with its own: 0.4 us of 11.5 for one token; of no use to the long units of PIPE 2)
-          if (PIPE == 1 && n == 0) m = largest();
+          if (PIPE == 1 && n == 0) m = largest() - Range<T>::RAISE;
           probabilities();
           const float top = largest();
-          const bool grow = top > m + TT_SLACK || (m == -INFINITY && top > -INFINITY);
+          const bool grow = top > m + (Range<T>::RAISE + Range<T>::SLACK) || (m == -INFINITY && top > -INFINITY);
           if (__any_sync(0xffffffffu, grow)) {
-            const float corr = grow ? ex2(m - top) : 1.f;  // 0 while the row has seen nothing
-            if (grow) m = top;
+            const float corr = grow ? ex2(m - (top - Range<T>::RAISE)) : 1.f;  // 0 while the row has seen nothing
+            if (grow) m = top - Range<T>::RAISE;
             l *= corr;
             if (n > 0) {
               // the product of tile n - 1: done when S of tile n + 1 is, which was issued after it

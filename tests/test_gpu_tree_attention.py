@@ -325,3 +325,18 @@ def test_other_workspaces_contents_do_not_matter(cuda_dev):
         outs.append(out.cpu())
     check(outs[0], reference(c), c)
     assert all(torch.equal(outs[0], o) for o in outs[1:])
+
+
+@pytest.mark.parametrize("page", [64, 20])
+@pytest.mark.parametrize("D,T,n,drop", [(64, 1, 32000, 17.34375), (128, 3, 32000, 17.34375), (64, 40, 131072, 17.34375),
+                                        (64, 1, 131072, 21.0), (128, 40, 40000, 19.5)])
+def test_many_small_probabilities_in_fp16(cuda_dev, D, T, n, drop, page):
+    """One key above many whose probabilities, e^-drop, lie below fp16's smallest step: together they still count. All
+    in one part, so that the one key's maximum holds for every other."""
+    c = make(50, 2, 1, D, page, [n], [T], "fp16", chain=True)
+    c["q"].zero_(), c["kc"].zero_(), c["vc"].fill_(1.0)
+    c["q"][:, :, 0] = 8.0
+    c["scale"] = 0.125
+    pg, r = int(c["table"][0, 777 // page]), 777 % page
+    c["kc"][pg, 0, r, 0], c["vc"][pg, 0, r] = drop, 0.0
+    check(run(cuda_dev, c, 1), reference(c), c)
