@@ -340,3 +340,81 @@ def test_many_small_probabilities_in_fp16(cuda_dev, D, T, n, drop, page):
     pg, r = int(c["table"][0, 777 // page]), 777 % page
     c["kc"][pg, 0, r, 0], c["vc"][pg, 0, r] = drop, 0.0
     check(run(cuda_dev, c, 1), reference(c), c)
+
+
+# ----------------------------------------------------------------------------- pages that are not multiples of 8
+@pytest.mark.parametrize("S", [1, 3])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("NQ,NKV,T", [(4, 2, 1), (8, 2, 4), (24, 3, 3), (8, 2, 8), (12, 3, 16), (10, 1, 7), (16, 2, 40)])
+def test_other_pages_every_block_shape(cuda_dev, NQ, NKV, T, D, S):
+    """2, 16, 24, 32, 64, 70 and 320 rows a KV head: every split of warps over rows and keys, odd numbers of rows."""
+    c = make(60 + T, NQ, NKV, D, 20, [500, 61, 0], [T, max(1, T - 1), 1], ("bf16", "fp16")[T % 2])
+    check(run(cuda_dev, c, S), reference(c), c)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_other_pages_queries_that_see_nothing(cuda_dev, D):
+    c = make(1, 8, 2, D, 20, [0, 0, 40], [5, 1, 3], "bf16")
+    c["mask"] = [0, 1, 0, 12, 0, 0, 0, 7, 0]
+    for S in (1, 2):
+        out = run(cuda_dev, c, S)
+        check(out, reference(c), c)
+        assert torch.count_nonzero(out[[0, 2, 4, 5]]) == 0
+
+
+@pytest.mark.parametrize("page", [20, 7])
+@pytest.mark.parametrize("D,dt,T", [(64, "bf16", 4), (64, "fp16", 7), (64, "bf16", 14), (64, "fp16", 64), (128, "bf16", 4),
+                                    (128, "fp16", 6), (128, "bf16", 16), (128, "fp16", 20)])
+def test_other_pages_masked_infinities_and_nans(cuda_dev, D, dt, T, page):
+    c = make(3, 8, 2, D, page, [70, 33], [T, 3], dt, spare=2)
+    k, v = c["kc"], c["vc"]
+    live = torch.zeros(k.shape[0], page, dtype=torch.bool)
+    for b, L in enumerate((70 + T, 36)):
+        for t in range(L):
+            live[c["table"][b, t // page], t % page] = True
+    k.transpose(1, 2)[~live] = float("nan")
+    v.transpose(1, 2)[~live] = float("inf")
+    poison = 70 + 2  # draft 2 of request 0
+    pg, r = int(c["table"][0, poison // page]), poison % page
+    v[pg, 0, r, 5], v[pg, 1, r, D - 1], k[pg, 0, r, 2] = float("inf"), float("nan"), float("nan")
+    sees = [bool((m >> 2) & 1) for m in c["mask"][:T]]
+    clean = dict(c, kc=k.clone(), vc=v.clone())
+    clean["kc"].nan_to_num_(0, 0, 0), clean["vc"].nan_to_num_(0, 0, 0)
+    for S in (1, 2):
+        out, ref = run(cuda_dev, c, S), reference(clean)
+        blind = [i for i in range(T) if not sees[i]] + list(range(T, T + 3))
+        check(out[blind], ref[blind], clean)
+        seeing = [i for i in range(T) if sees[i]]
+        assert not out[seeing, :4].isfinite().all(-1).any() and out[seeing, 4:, D - 1].isnan().all()
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_other_pages_outside_the_pool_and_past_max_q(cuda_dev, D):
+    c = make(4, 8, 2, D, 20, [100, 30], [4, 4], "bf16")
+    c["table"][0, 2], c["table"][1, 0] = -1, c["kc"].shape[0]
+    for S in (1, 2):
+        check(run(cuda_dev, c, S), reference(c), c)
+    c["ctx"][1] = 100000  # past the table: what the table holds
+    check(run(cuda_dev, c), reference(c), c)
+    c = make(5, 4, 1, D, 20, [20], [9], "bf16")
+    c["max_q"] = 6
+    out = run(cuda_dev, c)
+    assert out[6:].isnan().all()
+    check(out, tree_attention_f64(c["q"], c["kc"], c["vc"], c["table"], c["ctx"], c["cu"], c["mask"], c["scale"], 6), c)
+
+
+@pytest.mark.parametrize("D,dt,T,S", [(64, "bf16", 3, 1), (64, "fp16", 7, 3), (64, "bf16", 40, 2), (128, "fp16", 4, 3),
+                                      (128, "bf16", 8, 1), (128, "fp16", 16, 2), (128, "bf16", 64, 1)])
+@pytest.mark.parametrize("order", ["growing", "falling", "jumping"])
+def test_other_pages_maxima_that_move(cuda_dev, D, dt, T, S, order):
+    c = make(11, 8, 2, D, 20, [450, 130], [T, 2], dt)
+    direction = torch.randn(D, generator=torch.Generator().manual_seed(5))
+    direction /= direction.norm()
+    for b in range(2):
+        L = int(c["ctx"][b]) + (T if b == 0 else 2)
+        for t in range(L):
+            step = t // 16 if order == "growing" else -(t // 16) if order == "falling" else (t // 64) * 37 % 29
+            k = c["kc"][int(c["table"][b, t // 20]), :, t % 20]
+            k.copy_((0.2 * k.float() + 4.0 * step * direction).to(k.dtype))
+    c["q"] = (0.3 * c["q"].float() + 4.0 * direction).to(c["q"].dtype)
+    check(run(cuda_dev, c, S), reference(c), c)
