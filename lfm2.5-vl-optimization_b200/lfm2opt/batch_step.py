@@ -4,7 +4,7 @@ The batched sibling of decode_step.DecodeStep (batch 1, dense cache, argmax): th
 weights, and the four batched-serving operators in the order a serving loop runs them:
 
   kv_slots: a page and a slot for every active request's token
-  embedding -> per layer norm + quantization (add_rmsnorm_q), then either
+  embedding and first norm (embed_rmsnorm) -> per layer norm + quantization (add_rmsnorm_q), then either
     attention:  qkv GEMM -> qk_norm_rope_kv_paged (k, v into their slots) -> tree_attention (one query a request) -> o GEMM
     short conv: in_proj GEMM -> shortconv_step -> out_proj GEMM
   and w1|w3 GEMM with the SwiGLU -> w2 GEMM
@@ -85,7 +85,7 @@ class BatchDecodeStep:
         pos, slot = self.positions[at], torch.where(runs, self.slots[at], -1)
         K.embed_rmsnorm(self.tok, W.embed, W.norm[0], self.h, self.x, c.eps)
         codes = self._codes(c.hidden)
-        E.add_rmsnorm_q(self.h, None, W.norm[0], codes, self.s8, c.eps)
+        E.quant_rows(self.x, codes, self.s8)
         for i, L in enumerate(W.layer):
             if i in c.attn_layers:
                 E.gemm_i8(codes, self.s8, L["qkv"][0], L["qkv"][1], None, self.qkv, False)

@@ -148,3 +148,30 @@ def test_sampling_and_graph_replay(cuda_dev, weights):
         seen.append(a.tok.tolist())
     assert len({tuple(t) for t in seen}) > 1
     assert torch.equal(a.table, b.table) and all(torch.equal(a.kc[i], b.kc[i]) for i in a.kc)
+
+
+def test_every_norm_once(cuda_dev, weights):
+    """The first norm comes with the embedding: quantizing its rows gives the codes of norm and quantization in one, and
+    the step asks for the others, two a layer, only."""
+    s = BatchDecodeStep(weights, 3, 4, page=16, max_pages=2)
+    g = torch.Generator().manual_seed(6)
+    s.tok.copy_(torch.randint(0, CFG.vocab, (3,), generator=g))
+    s.active.fill_(1)
+    calls = []
+
+    class Spy:
+        def __getattr__(self, name, inner=s.E):
+            calls.append(name)
+            return getattr(inner, name)
+
+    s.E = Spy()
+    s.step()
+    assert calls.count("add_rmsnorm_q") == 2 * CFG.layers
+    e = dict(device=cuda_dev)
+    h, x = torch.empty(3, CFG.hidden, dtype=torch.bfloat16, **e), torch.empty(3, CFG.hidden, dtype=torch.bfloat16, **e)
+    tok = torch.randint(0, CFG.vocab, (3,), generator=g).to(cuda_dev)
+    a, b = [(torch.empty(3, CFG.hidden, dtype=torch.int8, **e), torch.empty(3, **e)) for _ in range(2)]
+    s.K.embed_rmsnorm(tok, weights.embed, weights.norm[0], h, x, CFG.eps)
+    s.E.quant_rows(x, *a)
+    s.E.add_rmsnorm_q(h, None, weights.norm[0], *b, CFG.eps)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
