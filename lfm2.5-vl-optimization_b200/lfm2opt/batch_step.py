@@ -133,7 +133,7 @@ class BatchDecodeStep:
         torch.cuda.current_stream(dev).wait_stream(side)
         self.active.copy_(active)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        with torch.cuda.graph(self.graph, stream=side):  # (its own stream may be one of another device)
             self.step()
         return self
 

@@ -143,7 +143,7 @@ class DecodeStep:
             self.step()
         torch.cuda.current_stream(dev).wait_stream(side)
         self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        with torch.cuda.graph(self.graph, stream=side):  # (its own stream may be one of another device)
             self.step()
         return self
 

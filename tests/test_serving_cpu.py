@@ -156,3 +156,40 @@ def test_arguments_in_one_block():
         refused("lfm2q_call_words", (code, pack(*swap(ok, **{f"_{number}": 1 << 32})), n), "32 bits")
     refused("lfm2q_call_words", (4, bytes(8 * 24), 13), "no such operator")
     refused("lfm2q_call_words", (0, None, 15), "number of arguments")
+
+
+@pytest.mark.parametrize("kind", ["BatchDecodeStep", "DecodeStep"])
+def test_a_step_is_captured_on_its_own_device(monkeypatch, kind):
+    """Without a stream torch.cuda.graph captures on one of the device that was current at the process's first capture;
+    the step's launches go to streams of the weights' device, and would run at once in place of being captured."""
+    import contextlib
+    from types import SimpleNamespace
+
+    from lfm2opt import batch_step, decode_step
+    dev, current, seen = torch.device("cuda", 1), [None], []
+
+    class Stream:
+        def __init__(self, device=None):
+            self.device = device
+
+        def wait_stream(self, other):
+            assert other.device == self.device == dev
+
+    @contextlib.contextmanager
+    def use(stream):
+        old, current[0] = current[0], stream
+        yield
+        current[0] = old
+
+    def graph(g, stream=None, **kw):
+        return use(stream if stream is not None else Stream(torch.device("cuda", 0)))
+
+    for name, fake in (("Stream", Stream), ("current_stream", Stream), ("stream", use), ("graph", graph),
+                       ("CUDAGraph", object)):
+        monkeypatch.setattr(torch.cuda, name, fake)
+    cls = getattr(batch_step if kind == "BatchDecodeStep" else decode_step, kind)
+    s = object.__new__(cls)
+    s.h, s.active = SimpleNamespace(device=dev), torch.ones(2, dtype=torch.int32)
+    s.step = lambda: seen.append(current[0].device)
+    assert s.capture() is s
+    assert seen == [dev, dev] and s.active.tolist() == [1, 1]
