@@ -41,8 +41,7 @@ int lfm2q_device_supported(void);
 /* Reads (and with clear != 0 resets) the sticky device error words that the tcgen05 GEMMs, the decode attention and the
  * tree attention set when one of their bounded pipeline waits gives up (no other kernel of this library waits on
  * anything but its own cluster's barriers). Returns LFM2Q_OK or LFM2Q_ETIMEOUT. Synchronous (copies three ints from the
- * device). Poll it after a batch of work
- * whose outputs matter. */
+ * device). Poll it after a batch of work whose outputs matter. */
 int lfm2q_check_device(int clear);
 
 /* ------------------------------------------------------------------ activation quantizers
@@ -268,7 +267,8 @@ int lfm2q_qk_norm_rope_kv_paged(const uint16_t *qkv, int64_t row_stride, const u
 /* Attention of drafted tokens over the paged cache. Request b brings the queries cu[b] .. cu[b + 1] of q [N, NQ, D] (1 to
  * max_q <= 64 of them: a tree, a chain, or one token), whose keys and values lie at its positions ctx[b] + j. Query i
  * sees every position < ctx[b], and ctx[b] + j where bit j of mask[cu[b] + i] is set (mask NULL: j <= i). out [N, NQ, D]
- * = softmax(scale q.k) v; a query that sees nothing gives zeros. Rows outside the requests, and those past max_q of a
+ * = softmax(scale q.k) v, in fp32 but for the probabilities, which are rounded to dtype before they meet v; a query that
+ * sees nothing gives zeros. Rows outside the requests, and those past max_q of a
  * request, are left as they were. NQ = G NKV, G <= 64; D 64 or 128; scale > 0. A position whose page is outside
  * [0, num_pages), or past the table, is not seen. B * NKV * (tiles of 128 rows, of whole queries, that max_q queries take)
  * * (max_pages * page / 64 + 8) must be below 2^31 - 2^16.
@@ -290,8 +290,8 @@ int lfm2q_tree_attention_splits(int B, int NQ, int NKV, int D, int max_q, int ma
  * theirs (>= 1 or NaN: all; always at least one), of those w_i >= min_p (of the largest, 1). tok[b] = the first index
  * whose running kept mass, in index order, exceeds u[b] (in [0, 1), values outside held to it, a NaN to 0) times the kept
  * mass. T <= 0 or NaN, a NaN among the logits, or none above -inf: the argmax, as lfm2q_argmax_next. A NULL temperature,
- * top_k, top_p or min_p [B] is off (temperature 1). Weights are summed as integers in steps of 2^-44 of the largest: the same token in any launch
- * shape. pos[0] += 1 if pos is not NULL. V <= 262144. */
+ * top_k, top_p or min_p [B] is off (temperature 1). Weights are summed as integers in steps of 2^-44 of the largest: the
+ * same token in any launch shape. pos[0] += 1 if pos is not NULL. V <= 262144. */
 int lfm2q_sample_next(const void *logits, int dtype, int64_t row_stride, const float *temperature, const int32_t *top_k,
                       const float *top_p, const float *min_p, const float *u, int64_t *tok, int64_t *pos, int B, int V,
                       void *stream);

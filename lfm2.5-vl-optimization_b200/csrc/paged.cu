@@ -23,8 +23,8 @@ namespace {
 // table) and barriers, so: the second scan (offsets without the refused requests) and the one of returned pages run only
 // where there are such, the search for a token's request runs in shared memory, and a small batch takes a small block.
 // Sums saturate at 2^31 - 1, past every limit (2^30 at most), and two of them add up within 32 bits. 37 requests x 16 tokens
-// and the removal of those that were not accepted (two calls, 11 KB): 9.8 us; 64 requests x 1024 tokens (1.1 MB; a second
-// kernel over the whole device writes the rows where there may be more than SL_FILL): 14 us for the two calls.
+// and the removal of those that were not accepted (two calls, 11 KB): 9.9 us; 64 requests x 1024 tokens (1.1 MB; a second
+// kernel over the whole device writes the rows where there may be more than SL_FILL): 14.8 us for the two calls.
 constexpr uint32_t SL_MAX = 0x7fffffffu;
 constexpr int SL_BIG = 1024;     // threads for batches of more than 256 requests
 constexpr int SL_FILL = 4096;    // token rows that the block fills itself
@@ -250,9 +250,20 @@ struct RopeArgs {
 // in the same lane. Everything in fp32 and rounded once; the angle positions[n] * inv_freq[i] is formed and reduced
 // in fp64 (exact product, then off by about n_turns * 2^-52): in fp32 a position of 10^6 would lose the angle's
 // fourth digit.
-// Bounded by HBM at many tokens (16384 tokens, 32 + 8 + 8 heads of 128: 67 us, 6.0 TB/s, 91 % of the measured copy rate):
-// there 128 threads with 6 pieces each in flight and 8 blocks an SM were fastest (256 x 4: 78 us, 128 x 3: 75 us). Few
-// tokens are latency: 384 threads with 2 pieces each (one token: 2.2 us against 3.4).
+// Two shapes of block, either for any number of heads (a block goes round its token's pieces until they are done): 128
+// threads with 6 pieces each in flight and 8 blocks an SM for many tokens, 384 threads with 2 for few, up to two tokens an
+// SM, where a token's latency counts. Both sides, many | few, half layout with norm, bf16, us:
+//            48 heads of 128   48 heads of 64   8 heads of 64   80 heads of 128
+//   1 token        4.9 | 3.1        3.4 | 2.3       2.2 | 2.2         8.0 | 4.3
+//   150            5.3 | 4.2        3.6 | 2.8       2.3 | 2.4         8.7 | 6.0
+//   300            6.5 | 5.8        3.9 | 3.5       2.3 | 2.5        11.9 | 9.7
+//   2000          20.0 | 19.0      10.6 | 11.4      4.3 | 7.0        33.1 | 30.9
+//   16384        113.9 | 118.7     56.3 | 71.2     25.6 | 48.6      204.5 | 207.2
+// The shapes were found on 16384 tokens with 48 heads of 128 in the interleaved layout (256 x 4: 78 us, 128 x 3: 75 us,
+// 128 x 6: 67 us, 6.0 TB/s, 91 % of the measured copy rate), where HBM bounds. The half layout, whose pairs lie in
+// two lanes, takes 114 us there (3.5 TB/s; 105 without the norm, as the interleaved one takes 60 in place of 68): eight
+// exchanges a piece. Few heads are bounded by a block's beginning: 8 heads of 64 leave half of the 128 threads without a
+// piece (26 us, 1.3 TB/s).
 struct RopeMany {
   static constexpr int T = 128, UN = 6, BLOCKS = 8;
 };

@@ -18,12 +18,14 @@
 // the sums show that the cut lies outside it, the row is done again by exact histograms: level by level, 1024 bins of
 // the order-preserving integer key inside the chosen bin, until a bin is one key.
 //
-// What bounds it: a pass over the staged row costs about 10 (counts) to 30 (weights in fp64) issue slots an element,
-// against 2 to 4 bytes to load; the cluster's four barriers and the sort are latency, some microseconds a row. Rows of
-// 65536: 256 in fp32 take 117 us with a nucleus alone (0.57 TB/s; two blocks an SM issue 2.2 instructions a clock and the
-// fp64 pipe is 18 % busy), in bf16 62 us unfiltered and 40 us with a top_k of 50 (no fp64 pass over the row); one row in
-// bf16 10.4 us. The list replaces an exact histogram over the whole row, several passes (16 rows with a top_k of 5000,
-// which still take them: 70 us). The other blocks leave before the list is sorted, so the next row starts on their SMs
+// What bounds it: instructions, against 2 to 4 bytes to load an element, and the latency of a row's phases (the cluster's
+// four barriers and the sort, some microseconds). 256 rows of 65536, in issue slots an element by counter: 132 in fp32 with
+// a nucleus alone (loads and maximum, counts, weights; 20 of them fp64), 75 in bf16 unfiltered (no counts), 47 in bf16 with
+// a top_k of 50 (no weights). They take 121 us (0.55 TB/s), 65 us and 43 us; two blocks an SM issue 2.3 to 2.4 instructions
+// a clock, the fp64 pipe is 18 %, 32 % and 1 % busy. min_p alone weighs every element too, 65 us. One row in bf16 10.7 us.
+// The list replaces an exact histogram over the whole row, several passes. Rows that still take them: 16 with a top_k of
+// 5000 39 us; 256 with a top_k of 50 at a temperature so low (0.05) that fewer tokens than that lie within 46 binary
+// orders of the largest 139 us. The other blocks leave before the list is sorted, so the next row starts on their SMs
 // (124 -> 120 us), and the whole block searches the piece that holds the token (120 -> 117; a warp did it before).
 #include <cooperative_groups.h>
 #include <cuda_fp16.h>

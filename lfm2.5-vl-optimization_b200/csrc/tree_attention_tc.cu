@@ -14,7 +14,8 @@
 // 2^11, as exact as below 1), rarely after the first tiles.
 //
 // What bounds it, by the rows a KV head has (bf16, 32 heads over 8 KV heads of 64, pages of 64). Few rows: the cache's
-// bytes. 64 requests x 1 token x 8000 positions: 185 us, 5.7 TB/s, 87 % of the measured copy rate; 32 requests x 16
+// bytes. 64 requests x 1 token x 8000 positions: 188 to 214 us from one allocation of the cache to the next, 4.9 to 5.6
+// TB/s, 75 to 85 % of the measured copy rate; 32 requests x 16
 // drafts x 500 to 4000 positions: 44 us, of which 30 at 5.0 TB/s, 4 until the first tile, 5 in the join. Many rows: the
 // softmax. 16 requests x 64 drafts x 8000 to 32000 positions: 305 us, 2.2 TB/s and 0.39 PFLOP/s; without its exponentials
 // the same loop took 243 us of 319, without the softmax 201 us. Two row tiles a block

@@ -11,7 +11,8 @@ weights, and the four batched-serving operators in the order a serving loop runs
   lm_head GEMM -> sample_next
 
 A step runs on the device without a synchronisation, so it captures into a CUDA graph (`capture`). A request that is not
-active, or for which there is no free page, sits the step out: its token, length and convolution states stay.
+active, for which there is no free page, or that holds max_pages full pages, sits the step out: its token, length and
+convolution states stay.
 """
 
 import torch
